@@ -356,6 +356,131 @@ B2D_API b2d_status b2d_debug_tune(b2d_ws* ws, int knob, int64_t value);
 B2D_API b2d_status b2d_test_gemm(const void* w_dev, int M, int K, const void* x_dev, int N, int epi,
                                  float* y_dev, const float* resid_dev, void* ybf_dev, int ldy, void* stream);
 
+/*
+ * ---- 4-bit paged KV cache ---------------------------------------------------
+ * Operators of their own (no model or workspace handle), for one layer's
+ * cache of any n_kv_heads and d_head 64 or 128; the batched step runs them on
+ * a workspace switched by b2d_workspace_kv_bits.  No reference counterpart.
+ *
+ * A position's row of one kv head is held in groups of 16 dims: a scale s, the
+ * smallest number >= max|x| / 7 with 5 exponent and 3 mantissa bits (its byte
+ * b is the half with the bits b << 7), at most 9216, and 16 codes
+ * clamp(round-to-nearest-even(x / s), -7, 7).  4.5 bits a value; held values
+ * are exact in bf16 and fp16.  Magnitudes above 64512 (infinities too) are
+ * held as 64512, NaN as 0.
+ *
+ * Pool: uint8 [num_blocks][n_kv_heads][18 * d_head], 16-byte aligned; a block
+ * holds 16 positions.  Within a kv head's 18 * d bytes (h < d / 64, g < 8,
+ * t < 4, p, q, e < 2, G < 4; code + 8 in a nibble, lower dims in lower bits):
+ *   K codes  [h][g][t][e][8 bytes]        position 8e + g, dims 64h + 16t ..
+ *   K scales [h][g][t][e]                 the same
+ *   V codes  [h][g][t][p][q][e][2 bytes]  position 8p + 2t + e, dims 64h + 8g + 4q ..
+ *   V scales [h][G][t][p][e]              position 8p + 2t + e, dims 64h + 16G ..
+ */
+typedef enum { B2D_F32 = 0, B2D_BF16 = 1, B2D_F16 = 2 } b2d_dtype;
+
+typedef struct {
+  void* pool;
+  const int32_t* table; /* [table_rows][blocks_per_seq]: block of positions 16i.. of each sequence */
+  uint32_t* status;     /* device word (or NULL) that the first bad input sets: 0x202 a position,
+                           length or row range, 0x203 a table row or entry; never cleared here */
+  int32_t n_kv_heads, d_head, num_blocks, blocks_per_seq, table_rows;
+  int32_t device;
+} b2d_kv4_cache;
+
+/* Rows to append.  Strides in elements; a head's dims are contiguous. */
+typedef struct {
+  const void *q, *k, *v; /* [n_rows][heads][d_head]; q may be NULL */
+  void* q_out;           /* the turned q (NULL with q); q itself, or apart from it */
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, q_out_row, q_out_head;
+  const int32_t* pos;    /* [n_rows]; < 0: the row is skipped, its q_out too */
+  const int32_t* seq;    /* [n_rows] table row of each row; NULL: row i has table row i */
+  const float *cos, *sin; /* [max_pos][rotary_dim / 2], or both NULL: no rotation */
+  int32_t dtype, q_out_dtype; /* b2d_dtype; they differ only with dtype = B2D_F32 */
+  int32_t n_rows, n_heads, rotary_dim, interleaved, max_pos;
+} b2d_kv4_rows;
+
+/*
+ * Turns q and k by their positions' angles (the first rotary_dim dims of a
+ * head; dims i and i + rotary_dim / 2 form a pair, or 2i and 2i + 1 when
+ * `interleaved`), writes the turned q to q_out, and writes k (turned) and v to
+ * the rows' positions in the cache.  The codes are those of the exact rotation
+ * of the given numbers (the kernel carries it to 47 bits).  A position that
+ * two rows of a call name receives either row's dims, in no particular order.
+ * Rows whose position lies past the table or the angles are skipped and set
+ * the status.
+ */
+B2D_API b2d_status b2d_kv4_append(const b2d_kv4_cache* cache, const b2d_kv4_rows* rows, void* stream);
+
+/* Rows out of the cache as values: k_dev, v_dev [n_rows][n_kv_heads][d_head]
+ * contiguous, `dtype`.  pos < 0 (and rows the table does not cover, which set
+ * the status) give zeros. */
+B2D_API b2d_status b2d_kv4_read(const b2d_kv4_cache* cache, const int32_t* pos_dev, const int32_t* seq_dev,
+                                int n_rows, int dtype, void* k_dev, void* v_dev, void* stream);
+
+/* Queries over the cache.  Strides in elements; a head's dims are contiguous. */
+typedef struct {
+  const void* q; /* [n_rows][n_heads][d_head], B2D_BF16 or B2D_F16 */
+  void* out;     /* the same shape and type; rows of no sequence stay as they are */
+  int64_t q_row, q_head, out_row, out_head;
+  const int32_t* lens;    /* [n_seqs] positions in the cache (0: rows see nothing) */
+  const int32_t* q_start; /* [n_seqs + 1] first row of each sequence; NULL: one row each */
+  int32_t dtype, n_rows, n_heads, n_seqs;
+  int32_t max_rows;       /* no sequence has more rows (1 when q_start is NULL) */
+  int32_t max_len;        /* no sequence is longer; at most 16 * blocks_per_seq */
+  float scale;            /* of the scores, usually d_head^-0.5 */
+} b2d_kv4_query;
+
+/*
+ * Causal attention: a sequence's n rows are its last n positions, row j of
+ * them sees positions 0 .. len - n + j.  A row that sees nothing is zero.
+ * Sequence i uses table row i; head h reads kv head h / (n_heads /
+ * n_kv_heads).  Products and sums in float32, probabilities rounded to q's
+ * type.  Results do not depend on the run: every sum has a fixed order.
+ * `scratch_dev` (16-byte aligned) holds the partial results of split
+ * sequences: b2d_kv4_attention_scratch says how many bytes, 0 for none.  Calls
+ * that may overlap need scratch of their own.
+ */
+B2D_API b2d_status b2d_kv4_attention_scratch(const b2d_kv4_cache* cache, const b2d_kv4_query* query,
+                                             uint64_t* bytes);
+B2D_API b2d_status b2d_kv4_attention(const b2d_kv4_cache* cache, const b2d_kv4_query* query, void* scratch_dev,
+                                     uint64_t scratch_bytes, void* stream);
+
+/*
+ * ---- logits adjustment --------------------------------------------------------
+ * What each row of a batch asks of its logits before a token is drawn
+ * (generate.py:32-39 has the repetition penalty alone, one value for a call).
+ * For row b, token v, with c_all and c_gen the times v occurs in
+ * history[b][0 .. hist_len) and history[b][prompt_len .. hist_len):
+ *   x = logits[b][v]
+ *   x = x > 0 ? x / rep : x * rep                      where c_all > 0
+ *   x = x - (frequency * c_gen + presence * [c_gen > 0])
+ *   x = x + bias_values[i]                             where bias_ids[i] = v
+ *   x = -infinity                                      where v's bit in allowed is 0
+ * An id that a row's biases list twice has the last one's value; ids outside
+ * the vocabulary count for nothing.  A row whose mask allows no token is
+ * -infinity throughout.  Any pointer but logits and out may be NULL: that rule
+ * is off (rep 1, the others 0; prompt_len 0; every token allowed).
+ */
+typedef struct {
+  const float* logits; /* [batch], rows logits_ld apart */
+  float* out;          /* rows out_ld apart; logits itself, or apart from it */
+  int64_t logits_ld, out_ld;
+  const int32_t* history;  /* [batch][hist_cap] */
+  const int32_t* hist_len; /* [batch], with history */
+  const int32_t* prompt_len; /* [batch]: the first entries, seen but not generated */
+  const float *rep, *presence, *frequency; /* [batch], with history */
+  const int32_t* bias_ids;   /* [batch][bias_cap] */
+  const float* bias_values;  /* [batch][bias_cap], with bias_ids */
+  const int32_t* bias_len;   /* [batch], with bias_ids */
+  const uint32_t* allowed;   /* [batch][allowed_ld] words: token v is bit v % 32 of word v / 32 */
+  int64_t allowed_ld;
+  int32_t batch, vocab, hist_cap, bias_cap;
+  int32_t device;
+} b2d_logits_rules;
+
+B2D_API b2d_status b2d_adjust_logits(const b2d_logits_rules* rules, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

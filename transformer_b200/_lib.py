@@ -58,6 +58,42 @@ class Sampling(ctypes.Structure):
                 ("rep_penalty", ctypes.c_double)]
 
 
+# b2d_dtype
+B2D_F32, B2D_BF16, B2D_F16 = 0, 1, 2
+
+
+class Kv4Cache(ctypes.Structure):
+    _fields_ = [("pool", ctypes.c_void_p), ("table", ctypes.c_void_p), ("status", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int32) for n in ("n_kv_heads", "d_head", "num_blocks", "blocks_per_seq", "table_rows",
+                                              "device")]
+
+
+class Kv4Rows(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("q", "k", "v", "q_out")] + \
+               [(n, ctypes.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "q_out_row",
+                                              "q_out_head")] + \
+               [(n, ctypes.c_void_p) for n in ("pos", "seq", "cos", "sin")] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "q_out_dtype", "n_rows", "n_heads", "rotary_dim",
+                                              "interleaved", "max_pos")]
+
+
+class Kv4Query(ctypes.Structure):
+    _fields_ = [("q", ctypes.c_void_p), ("out", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int64) for n in ("q_row", "q_head", "out_row", "out_head")] + \
+               [("lens", ctypes.c_void_p), ("q_start", ctypes.c_void_p)] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "n_rows", "n_heads", "n_seqs", "max_rows", "max_len")] + \
+               [("scale", ctypes.c_float)]
+
+
+class LogitsRules(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("out", ctypes.c_void_p), ("logits_ld", ctypes.c_int64),
+                ("out_ld", ctypes.c_int64)] + \
+               [(n, ctypes.c_void_p) for n in ("history", "hist_len", "prompt_len", "rep", "presence", "frequency",
+                                               "bias_ids", "bias_values", "bias_len", "allowed")] + \
+               [("allowed_ld", ctypes.c_int64)] + \
+               [(n, ctypes.c_int32) for n in ("batch", "vocab", "hist_cap", "bias_cap", "device")]
+
+
 #: every symbol include/b2d.h declares, with (restype, argtypes)
 _P = ctypes.c_void_p
 _SIGS = {
@@ -97,6 +133,13 @@ _SIGS = {
     "b2d_debug_tune": (ctypes.c_int, [_P, ctypes.c_int, ctypes.c_int64]),
     "b2d_test_gemm": (ctypes.c_int, [_P, ctypes.c_int, ctypes.c_int, _P, ctypes.c_int, ctypes.c_int, _P, _P, _P,
                                      ctypes.c_int, _P]),
+    "b2d_kv4_append": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4Rows), _P]),
+    "b2d_kv4_read": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), _P, _P, ctypes.c_int, ctypes.c_int, _P, _P, _P]),
+    "b2d_kv4_attention_scratch": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4Query),
+                                                 ctypes.POINTER(ctypes.c_uint64)]),
+    "b2d_kv4_attention": (ctypes.c_int, [ctypes.POINTER(Kv4Cache), ctypes.POINTER(Kv4Query), _P, ctypes.c_uint64,
+                                         _P]),
+    "b2d_adjust_logits": (ctypes.c_int, [ctypes.POINTER(LogitsRules), _P]),
 }
 
 _lib = None

@@ -14,6 +14,7 @@
 
 #include "../../include/b2d.h"
 #include "attn_paged.cuh"
+#include "b2d_host.h"
 #include "batched.cuh"
 #include "decode_b1.cuh"
 #include "decode_b1c.cuh"
@@ -30,6 +31,12 @@ b2d_status cuda_fail(cudaError_t e, const char* what) {
   if (e == cudaErrorCooperativeLaunchTooLarge) return B2D_ERR_LAUNCH;
   return B2D_ERR_CUDA;
 }
+
+}  // namespace
+
+b2d_status b2d::cuda_failed(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+
+namespace {
 
 #define B2D_CUDA(call, what)                         \
   do {                                               \

@@ -1,0 +1,224 @@
+// kv4.cu — launches of the 4-bit KV cache's kernels and their C entry points
+// (b2d_kv4_* in include/b2d.h).
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+
+#include "b2d_host.h"
+#include "kv4.cuh"
+
+namespace b2d {
+
+namespace {
+
+template <class T, class TQ>
+cudaError_t append_typed(const Kv4AppendArgs& a, cudaStream_t st, bool pdl) {
+  const int slices = kKv4AppendThreads / (a.c.d / kKv4Group);
+  const int total = (a.q ? a.n_heads : 0) + 2 * a.c.n_kv;
+  // one head a thread until the rows alone fill the GPU's threads several times over
+  const int heads = a.n_rows >= 2048 ? total : slices;
+  const dim3 grid(static_cast<unsigned>(a.n_rows), static_cast<unsigned>((total + heads - 1) / heads));
+  return launch(kv4_append_kernel<T, TQ>, grid, dim3(kKv4AppendThreads), 0, st, pdl, a, heads);
+}
+
+template <class Op, int NH, int NB>
+cudaError_t attn_shape(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
+  const int64_t units = static_cast<int64_t>(a.n_seqs) * a.c.n_kv * a.tiles;
+  cudaError_t e = launch(kv4_attn_kernel<Op, NH, NB>, dim3(static_cast<unsigned>(units * a.splits)),
+                         dim3(32 * kKv4Warps), 0, st, pdl, a);
+  if (e == cudaSuccess && a.splits > 1)
+    e = launch(kv4_join_kernel<Op, NH, NB>, dim3(static_cast<unsigned>((units * 8 * NB + 7) / 8)), dim3(256), 0, st,
+               true, a);
+  return e;
+}
+
+template <class Op>
+cudaError_t attn_typed(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
+  const bool wide = a.tile_cols > 8;
+  if (a.c.d == 64) return wide ? attn_shape<Op, 1, 2>(a, st, pdl) : attn_shape<Op, 1, 1>(a, st, pdl);
+  return wide ? attn_shape<Op, 2, 2>(a, st, pdl) : attn_shape<Op, 2, 1>(a, st, pdl);
+}
+
+}  // namespace
+
+cudaError_t kv4_append(const Kv4AppendArgs& a, cudaStream_t st, bool pdl) {
+  if (a.n_rows == 0) return cudaSuccess;
+  if (a.dtype == B2D_F32) {
+    if (a.q_out_dtype == B2D_F32) return append_typed<float, float>(a, st, pdl);
+    if (a.q_out_dtype == B2D_F16) return append_typed<float, __half>(a, st, pdl);
+    return append_typed<float, __nv_bfloat16>(a, st, pdl);
+  }
+  if (a.dtype == B2D_F16) return append_typed<__half, __half>(a, st, pdl);
+  return append_typed<__nv_bfloat16, __nv_bfloat16>(a, st, pdl);
+}
+
+cudaError_t kv4_read(const Kv4ReadArgs& a, cudaStream_t st) {
+  const int64_t n = static_cast<int64_t>(a.n_rows) * a.c.n_kv * 2 * (a.c.d / kKv4Group);
+  if (n == 0) return cudaSuccess;
+  const dim3 grid(static_cast<unsigned>((n + 255) / 256)), block(256);
+  if (a.dtype == B2D_F32) return launch(kv4_read_kernel<float>, grid, block, 0, st, false, a);
+  if (a.dtype == B2D_F16) return launch(kv4_read_kernel<__half>, grid, block, 0, st, false, a);
+  return launch(kv4_read_kernel<__nv_bfloat16>, grid, block, 0, st, false, a);
+}
+
+void kv4_attn_plan(Kv4AttnArgs& a, int sms) {
+  const int64_t cols = static_cast<int64_t>(a.max_rows) * (a.n_heads / a.c.n_kv);
+  a.tile_cols = cols <= 8 ? 8 : 16;
+  a.tiles = static_cast<int>((cols + a.tile_cols - 1) / a.tile_cols);
+  const int pages = std::max(1, (a.max_len + kKv4Page - 1) / kKv4Page);
+  const int64_t units = static_cast<int64_t>(a.n_seqs) * a.c.n_kv * a.tiles;
+  // enough CTAs for the GPU, at least 8 pages (two a warp) each
+  const int64_t want = std::max<int64_t>(1, int64_t(sms) * 4 / std::max<int64_t>(1, units));
+  const int64_t splits = std::min<int64_t>(want, std::max(1, pages / 8));
+  a.split_pages = static_cast<int>((pages + splits - 1) / splits);
+  a.splits = (pages + a.split_pages - 1) / a.split_pages;
+}
+
+uint64_t kv4_attn_scratch(const Kv4AttnArgs& a) {
+  if (a.splits <= 1) return 0;
+  return uint64_t(a.n_seqs) * a.c.n_kv * a.tiles * a.splits * a.tile_cols * (a.c.d + 4) * sizeof(float);
+}
+
+cudaError_t kv4_attention(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
+  if (a.n_rows == 0 || a.n_seqs == 0) return cudaSuccess;
+  return a.dtype == B2D_F16 ? attn_typed<Kv4Half>(a, st, pdl) : attn_typed<Kv4Bf16>(a, st, pdl);
+}
+
+}  // namespace b2d
+
+namespace {
+
+#define KV4_CUDA(call, what)                              \
+  do {                                                    \
+    cudaError_t e_ = (call);                              \
+    if (e_ != cudaSuccess) return b2d::cuda_failed(e_, what); \
+  } while (0)
+
+constexpr int64_t kMaxBlocks = 0x7fffffff;  // CTAs of a launch
+
+b2d_status check_cache(const b2d_kv4_cache* c, b2d::Kv4Cache& k) {
+  if (!c || !c->pool || (reinterpret_cast<uintptr_t>(c->pool) & 15u) || !c->table || c->n_kv_heads < 1 ||
+      c->num_blocks < 1 || c->blocks_per_seq < 1 || c->table_rows < 1 || c->device < 0)
+    return B2D_ERR_INVALID_ARG;
+  if (c->d_head != 64 && c->d_head != 128) return B2D_ERR_UNSUPPORTED;
+  if (c->blocks_per_seq > 0x7fffffff / b2d::kKv4Page) return B2D_ERR_INVALID_ARG;
+  k.pool = static_cast<uint8_t*>(c->pool);
+  k.table = c->table;
+  k.status = c->status;
+  k.n_kv = c->n_kv_heads;
+  k.d = c->d_head;
+  k.num_blocks = c->num_blocks;
+  k.bps = c->blocks_per_seq;
+  k.table_rows = c->table_rows;
+  k.table_ld = c->blocks_per_seq;
+  return B2D_OK;
+}
+
+b2d_status check_query(const b2d_kv4_cache* c, const b2d_kv4_query* q, b2d::Kv4AttnArgs& a) {
+  std::memset(&a, 0, sizeof(a));
+  const b2d_status s = check_cache(c, a.c);
+  if (s != B2D_OK) return s;
+  if (!q || !q->q || !q->out || !q->lens || q->n_rows < 0 || q->n_seqs < 0 || q->n_heads < 1 ||
+      q->n_heads % c->n_kv_heads || q->max_rows < 1 || q->n_seqs > c->table_rows || q->max_len < 0 ||
+      int64_t(q->max_len) > int64_t(c->blocks_per_seq) * b2d::kKv4Page || !(q->scale > 0.f) || std::isinf(q->scale) ||
+      (!q->q_start && (q->n_rows != q->n_seqs || q->max_rows != 1)))
+    return B2D_ERR_INVALID_ARG;
+  if (q->dtype != B2D_BF16 && q->dtype != B2D_F16) return B2D_ERR_UNSUPPORTED;
+  a.q = q->q;
+  a.out = q->out;
+  a.q_row = q->q_row; a.q_head = q->q_head;
+  a.o_row = q->out_row; a.o_head = q->out_head;
+  a.lens = q->lens;
+  a.q_start = q->q_start;
+  a.scale_log2 = q->scale * 1.4426950408889634f;
+  a.n_rows = q->n_rows;
+  a.n_heads = q->n_heads;
+  a.n_seqs = q->n_seqs;
+  a.max_rows = std::min(q->max_rows, std::max(1, q->n_rows));
+  a.max_len = q->max_len;
+  a.dtype = q->dtype;
+  int sms = 0;
+  const cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c->device);
+  if (e != cudaSuccess) return b2d::cuda_failed(e, "SM count");
+  b2d::kv4_attn_plan(a, sms);
+  if (int64_t(a.n_seqs) * a.c.n_kv * a.tiles * a.splits > kMaxBlocks) return B2D_ERR_UNSUPPORTED;
+  return B2D_OK;
+}
+
+}  // namespace
+
+extern "C" b2d_status b2d_kv4_append(const b2d_kv4_cache* cache, const b2d_kv4_rows* rows, void* stream) {
+  b2d::Kv4AppendArgs a;
+  std::memset(&a, 0, sizeof(a));
+  const b2d_status s = check_cache(cache, a.c);
+  if (s != B2D_OK) return s;
+  if (!rows || !rows->k || !rows->v || !rows->pos ||
+      (rows->q && rows->q == rows->q_out &&
+       (rows->q_row != rows->q_out_row || rows->q_head != rows->q_out_head || rows->dtype != rows->q_out_dtype)) || rows->n_rows < 0 || (rows->q != nullptr) != (rows->q_out != nullptr) ||
+      (rows->q && rows->n_heads < 1) || (rows->cos != nullptr) != (rows->sin != nullptr) ||
+      (rows->cos && (rows->rotary_dim < 2 || rows->rotary_dim > cache->d_head || rows->rotary_dim % 2 ||
+                     rows->max_pos < 1)) ||
+      (!rows->seq && rows->n_rows > cache->table_rows))
+    return B2D_ERR_INVALID_ARG;
+  const bool same = rows->q_out_dtype == rows->dtype;
+  if (rows->dtype < B2D_F32 || rows->dtype > B2D_F16 || rows->q_out_dtype < B2D_F32 || rows->q_out_dtype > B2D_F16 ||
+      (rows->q && !same && rows->dtype != B2D_F32))
+    return B2D_ERR_UNSUPPORTED;
+  a.q = rows->q; a.k = rows->k; a.v = rows->v; a.q_out = rows->q_out;
+  a.q_row = rows->q_row; a.q_head = rows->q_head; a.k_row = rows->k_row; a.k_head = rows->k_head;
+  a.v_row = rows->v_row; a.v_head = rows->v_head; a.qo_row = rows->q_out_row; a.qo_head = rows->q_out_head;
+  a.pos = rows->pos; a.seq = rows->seq; a.cos = rows->cos; a.sin = rows->sin;
+  a.n_rows = rows->n_rows; a.n_heads = rows->q ? rows->n_heads : 0;
+  a.rotary = rows->cos ? rows->rotary_dim : 0;
+  a.interleaved = rows->interleaved != 0;
+  a.max_pos = rows->max_pos;
+  a.dtype = rows->dtype;
+  a.q_out_dtype = rows->q ? rows->q_out_dtype : rows->dtype;
+  b2d::DeviceScope dev(cache->device);
+  KV4_CUDA(dev.error(), "device");
+  KV4_CUDA(b2d::kv4_append(a, static_cast<cudaStream_t>(stream), false), "kv4 append");
+  return B2D_OK;
+}
+
+extern "C" b2d_status b2d_kv4_read(const b2d_kv4_cache* cache, const int32_t* pos_dev, const int32_t* seq_dev,
+                                   int n_rows, int dtype, void* k_dev, void* v_dev, void* stream) {
+  b2d::Kv4ReadArgs a;
+  std::memset(&a, 0, sizeof(a));
+  const b2d_status s = check_cache(cache, a.c);
+  if (s != B2D_OK) return s;
+  if (!pos_dev || !k_dev || !v_dev || n_rows < 0 || (!seq_dev && n_rows > cache->table_rows)) return B2D_ERR_INVALID_ARG;
+  if (dtype < B2D_F32 || dtype > B2D_F16) return B2D_ERR_UNSUPPORTED;
+  if (int64_t(n_rows) * a.c.n_kv * 2 * (a.c.d / b2d::kKv4Group) > kMaxBlocks * 256) return B2D_ERR_UNSUPPORTED;
+  a.k = k_dev; a.v = v_dev; a.pos = pos_dev; a.seq = seq_dev;
+  a.n_rows = n_rows;
+  a.dtype = dtype;
+  b2d::DeviceScope dev(cache->device);
+  KV4_CUDA(dev.error(), "device");
+  KV4_CUDA(b2d::kv4_read(a, static_cast<cudaStream_t>(stream)), "kv4 read");
+  return B2D_OK;
+}
+
+extern "C" b2d_status b2d_kv4_attention_scratch(const b2d_kv4_cache* cache, const b2d_kv4_query* query,
+                                                uint64_t* bytes) {
+  if (!bytes) return B2D_ERR_INVALID_ARG;
+  *bytes = 0;
+  b2d::Kv4AttnArgs a;
+  const b2d_status s = check_query(cache, query, a);
+  if (s == B2D_OK) *bytes = b2d::kv4_attn_scratch(a);
+  return s;
+}
+
+extern "C" b2d_status b2d_kv4_attention(const b2d_kv4_cache* cache, const b2d_kv4_query* query, void* scratch_dev,
+                                        uint64_t scratch_bytes, void* stream) {
+  b2d::Kv4AttnArgs a;
+  const b2d_status s = check_query(cache, query, a);
+  if (s != B2D_OK) return s;
+  const uint64_t need = b2d::kv4_attn_scratch(a);
+  if (need > 0 && (!scratch_dev || (reinterpret_cast<uintptr_t>(scratch_dev) & 15u) || scratch_bytes < need))
+    return B2D_ERR_INVALID_ARG;
+  a.part = static_cast<float*>(scratch_dev);
+  b2d::DeviceScope dev(cache->device);
+  KV4_CUDA(dev.error(), "device");
+  KV4_CUDA(b2d::kv4_attention(a, static_cast<cudaStream_t>(stream), false), "kv4 attention");
+  return B2D_OK;
+}

@@ -37,6 +37,7 @@ import torch
 
 from . import _lib
 from .config import ModelConfig
+from .kv4 import _stream_on
 from .multi_sm_decode import DecodeEngine, _ptr, _stream_ptr
 from .packing import prepare_decode_weights_nlayer
 
@@ -71,6 +72,74 @@ class Sampler:
                                  _ptr(self.out), _stream_ptr(stream))
         _lib.check(st, "b2d_sample")
         return self.out[:batch]
+
+
+def adjust_logits(logits, *, out=None, history=None, hist_len=None, prompt_len=None, rep_penalty=None,
+                  presence=None, frequency=None, bias_ids=None, bias_values=None, bias_len=None, allowed=None,
+                  stream=None) -> torch.Tensor:
+    """Each row's own rules on a batch of logits (``b2d_adjust_logits``): what a
+    request asks of its tokens before one is drawn.  ``logits``: float32
+    [batch, vocab] on a GPU, rows contiguous; returns ``out`` (default: a new
+    tensor; ``logits`` itself adjusts in place).  Async, stream-ordered.
+
+    * ``history`` int32 [batch, cap] with ``hist_len`` int32 [batch]: the tokens
+      of each row so far, of which the first ``prompt_len`` [batch] (default 0)
+      were given and the rest generated;
+    * ``rep_penalty`` float32 [batch]: logits of tokens seen are divided (those
+      above 0) or multiplied by it;
+    * ``frequency``, ``presence`` float32 [batch]: subtracted from the logits of
+      generated tokens, times their count and once;
+    * ``bias_ids`` int32 [batch, n], ``bias_values`` float32 [batch, n],
+      ``bias_len`` int32 [batch]: added to the logits of these tokens (an id
+      listed twice: the last one counts);
+    * ``allowed`` int32 [batch, >= ceil(vocab / 32)]: token v is bit v % 32 of
+      word v // 32; tokens whose bit is 0 become -infinity.
+
+    In this order; ids outside the vocabulary count for nothing."""
+    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.device.type != "cuda" or logits.shape[1] < 1 or (
+            logits.stride(1) != 1 and logits.shape[1] > 1):
+        raise ValueError("logits must be float32 [batch, vocab] with contiguous rows on a GPU")
+    dev, (batch, vocab) = logits.device, logits.shape
+    if out is None:
+        with torch.cuda.stream(stream or torch.cuda.current_stream(dev)):
+            out = torch.empty(batch, vocab, dtype=torch.float32, device=dev)
+    elif (out.dtype != torch.float32 or out.shape != logits.shape or out.device != dev
+          or (out.stride(1) != 1 and vocab > 1)):
+        raise ValueError("out must be float32 like logits")
+
+    def take(t, name, dtype, shape):
+        if t is None:
+            return None
+        if t.dtype != dtype or t.device != dev or t.dim() != len(shape) or not t.is_contiguous() or any(
+                n is not None and t.shape[i] != n for i, n in enumerate(shape)):
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor on {dev} of shape "
+                             f"{[n if n is not None else 'any' for n in shape]}")
+        return t.data_ptr()
+
+    if (history is None) != (hist_len is None):
+        raise ValueError("history and hist_len go together")
+    if history is None and any(t is not None for t in (prompt_len, rep_penalty, presence, frequency)):
+        raise ValueError("penalties need the history")
+    if (bias_ids is None) != (bias_values is None) or (bias_ids is None) != (bias_len is None):
+        raise ValueError("bias_ids, bias_values and bias_len go together")
+    if allowed is not None and (allowed.dim() != 2 or allowed.shape[1] < (vocab + 31) // 32):
+        raise ValueError(f"allowed must have {(vocab + 31) // 32} words a row")
+    n_bias = bias_ids.shape[-1] if bias_ids is not None else 0
+    r = _lib.LogitsRules(
+        logits.data_ptr(), out.data_ptr(), logits.stride(0) if batch > 1 else vocab,
+        out.stride(0) if batch > 1 else vocab,
+        take(history, "history", torch.int32, (batch, None)), take(hist_len, "hist_len", torch.int32, (batch,)),
+        take(prompt_len, "prompt_len", torch.int32, (batch,)),
+        take(rep_penalty, "rep_penalty", torch.float32, (batch,)),
+        take(presence, "presence", torch.float32, (batch,)),
+        take(frequency, "frequency", torch.float32, (batch,)),
+        take(bias_ids, "bias_ids", torch.int32, (batch, None)),
+        take(bias_values, "bias_values", torch.float32, (batch, n_bias)),
+        take(bias_len, "bias_len", torch.int32, (batch,)),
+        take(allowed, "allowed", torch.int32, (batch, None)), allowed.shape[1] if allowed is not None else 0,
+        batch, vocab, history.shape[1] if history is not None else 0, n_bias, dev.index or 0)
+    _lib.check(_lib.load().b2d_adjust_logits(ctypes.byref(r), _stream_on(stream, dev)), "b2d_adjust_logits")
+    return out
 
 
 _SAMPLERS: dict = {}
