@@ -37,7 +37,7 @@ import torch
 
 from . import _lib
 from .config import ModelConfig
-from .kv4 import _stream_on
+from .kv4 import _empty, _stream_on
 from .multi_sm_decode import DecodeEngine, _ptr, _stream_ptr
 from .packing import prepare_decode_weights_nlayer
 
@@ -96,48 +96,46 @@ def adjust_logits(logits, *, out=None, history=None, hist_len=None, prompt_len=N
       word v // 32; tokens whose bit is 0 become -infinity.
 
     In this order; ids outside the vocabulary count for nothing."""
-    if logits.dtype != torch.float32 or logits.dim() != 2 or logits.device.type != "cuda" or logits.shape[1] < 1 or (
-            logits.stride(1) != 1 and logits.shape[1] > 1):
-        raise ValueError("logits must be float32 [batch, vocab] with contiguous rows on a GPU")
-    dev, (batch, vocab) = logits.device, logits.shape
+    dev = logits.device
+    if logits.dtype != torch.float32 or logits.dim() != 2 or dev.type != "cuda":
+        raise ValueError("logits must be float32 [batch, vocab] on a GPU")
+    batch, vocab = logits.shape
     if out is None:
-        with torch.cuda.stream(stream or torch.cuda.current_stream(dev)):
-            out = torch.empty(batch, vocab, dtype=torch.float32, device=dev)
-    elif (out.dtype != torch.float32 or out.shape != logits.shape or out.device != dev
-          or (out.stride(1) != 1 and vocab > 1)):
-        raise ValueError("out must be float32 like logits")
-
-    def take(t, name, dtype, shape):
-        if t is None:
-            return None
-        if t.dtype != dtype or t.device != dev or t.dim() != len(shape) or not t.is_contiguous() or any(
-                n is not None and t.shape[i] != n for i, n in enumerate(shape)):
-            raise ValueError(f"{name} must be a contiguous {dtype} tensor on {dev} of shape "
-                             f"{[n if n is not None else 'any' for n in shape]}")
-        return t.data_ptr()
-
+        out = _empty(logits.shape, torch.float32, dev, stream)
+    ld, out_ld = logits.stride(0) if batch > 1 else vocab, out.stride(0) if batch > 1 else vocab
+    if vocab < 1 or out.dtype != torch.float32 or out.shape != logits.shape or out.device != dev or (
+            vocab > 1 and (logits.stride(1) != 1 or out.stride(1) != 1)) or min(ld, out_ld) < vocab:
+        raise ValueError("logits and out must be float32 [batch, vocab] on one GPU, their rows contiguous and apart")
     if (history is None) != (hist_len is None):
         raise ValueError("history and hist_len go together")
-    if history is None and any(t is not None for t in (prompt_len, rep_penalty, presence, frequency)):
+    if history is None and not (prompt_len is None and rep_penalty is None and presence is None and frequency is None):
         raise ValueError("penalties need the history")
     if (bias_ids is None) != (bias_values is None) or (bias_ids is None) != (bias_len is None):
         raise ValueError("bias_ids, bias_values and bias_len go together")
-    if allowed is not None and (allowed.dim() != 2 or allowed.shape[1] < (vocab + 31) // 32):
-        raise ValueError(f"allowed must have {(vocab + 31) // 32} words a row")
+    one = (batch,)
+    cap = history.shape[-1] if history is not None else 0
     n_bias = bias_ids.shape[-1] if bias_ids is not None else 0
-    r = _lib.LogitsRules(
-        logits.data_ptr(), out.data_ptr(), logits.stride(0) if batch > 1 else vocab,
-        out.stride(0) if batch > 1 else vocab,
-        take(history, "history", torch.int32, (batch, None)), take(hist_len, "hist_len", torch.int32, (batch,)),
-        take(prompt_len, "prompt_len", torch.int32, (batch,)),
-        take(rep_penalty, "rep_penalty", torch.float32, (batch,)),
-        take(presence, "presence", torch.float32, (batch,)),
-        take(frequency, "frequency", torch.float32, (batch,)),
-        take(bias_ids, "bias_ids", torch.int32, (batch, None)),
-        take(bias_values, "bias_values", torch.float32, (batch, n_bias)),
-        take(bias_len, "bias_len", torch.int32, (batch,)),
-        take(allowed, "allowed", torch.int32, (batch, None)), allowed.shape[1] if allowed is not None else 0,
-        batch, vocab, history.shape[1] if history is not None else 0, n_bias, dev.index or 0)
+    words = allowed.shape[-1] if allowed is not None else 0
+    if allowed is not None and 32 * words < vocab:
+        raise ValueError(f"allowed must have {(vocab + 31) // 32} words a row")
+    ptrs = []
+    for t, name, dtype, shape in (
+            (history, "history", torch.int32, (batch, cap)), (hist_len, "hist_len", torch.int32, one),
+            (prompt_len, "prompt_len", torch.int32, one), (rep_penalty, "rep_penalty", torch.float32, one),
+            (presence, "presence", torch.float32, one), (frequency, "frequency", torch.float32, one),
+            (bias_ids, "bias_ids", torch.int32, (batch, n_bias)),
+            (bias_values, "bias_values", torch.float32, (batch, n_bias)), (bias_len, "bias_len", torch.int32, one),
+            (allowed, "allowed", torch.int32, (batch, words))):
+        if t is None:
+            ptrs.append(None)
+        elif t.dtype != dtype or t.shape != shape or t.device != dev or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on {dev}")
+        else:
+            ptrs.append(t.data_ptr())
+    if not batch:
+        return out
+    r = _lib.LogitsRules(logits.data_ptr(), out.data_ptr(), ld, out_ld, *ptrs, words, batch, vocab, cap, n_bias,
+                         dev.index)
     _lib.check(_lib.load().b2d_adjust_logits(ctypes.byref(r), _stream_on(stream, dev)), "b2d_adjust_logits")
     return out
 

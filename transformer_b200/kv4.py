@@ -26,9 +26,17 @@ PAGE_TOKENS = 16  # positions per block
 _TYPES = {torch.float32: _lib.B2D_F32, torch.bfloat16: _lib.B2D_BF16, torch.float16: _lib.B2D_F16}
 
 
-def _stream_on(stream, device) -> ctypes.c_void_p:
+def _stream_on(stream, device) -> int:
     """The stream's handle, by default the current one of ``device``."""
-    return ctypes.c_void_p((stream or torch.cuda.current_stream(device)).cuda_stream)
+    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _empty(shape, dtype, device, stream) -> torch.Tensor:
+    """A tensor from the stream's own memory (as torch's allocator keeps it)."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def page_bytes(d_head: int) -> int:
@@ -51,33 +59,44 @@ def check_status(status: torch.Tensor) -> None:
 
 
 def _ints(t, name, device, n):
-    if t.dtype != torch.int32 or t.device != device or t.dim() != 1 or not t.is_contiguous() or t.numel() != n:
+    if t.dtype != torch.int32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous int32 tensor of {n} items on {device}")
     return t.data_ptr()
 
 
 def _cache(pool, table, status, n_kv, d) -> _lib.Kv4Cache:
-    if pool.device.type != "cuda":
+    dev = pool.device
+    if dev.type != "cuda":
         raise ValueError("pool must be on a GPU")
-    if pool.dtype != torch.uint8 or pool.dim() != 3 or not pool.is_contiguous() or tuple(pool.shape[1:]) != (
-            n_kv, page_bytes(d)) or pool.shape[0] < 1:
-        raise ValueError(f"pool must be contiguous uint8 [num_blocks, {n_kv}, {page_bytes(d)}] (see new_kv4_pool)")
-    if table.dtype != torch.int32 or table.device != pool.device or table.dim() != 2 or not table.is_contiguous() or (
+    blocks = pool.shape[0]
+    if pool.dtype != torch.uint8 or pool.shape != (blocks, n_kv, 18 * d) or blocks < 1 or not pool.is_contiguous():
+        raise ValueError(f"pool must be contiguous uint8 [num_blocks, {n_kv}, {18 * d}] (see new_kv4_pool)")
+    if table.dtype != torch.int32 or table.dim() != 2 or table.device != dev or not table.is_contiguous() or (
             table.numel() < 1):
         raise ValueError("table must be a contiguous int32 [n_seqs, blocks_per_seq] tensor on the pool's device")
-    if status is not None and (status.dtype != torch.int32 or status.device != pool.device or status.numel() != 1):
+    if status is not None and (status.dtype != torch.int32 or status.device != dev or status.numel() != 1):
         raise ValueError("status must be an int32 tensor of one item on the pool's device")
-    return _lib.Kv4Cache(pool.data_ptr(), table.data_ptr(), status.data_ptr() if status is not None else None, n_kv, d,
-                         pool.shape[0], table.shape[1], table.shape[0], pool.device.index or 0)
+    rows, bps = table.shape
+    return _lib.Kv4Cache(pool.data_ptr(), table.data_ptr(), None if status is None else status.data_ptr(), n_kv, d,
+                         blocks, bps, rows, dev.index)
 
 
-def _heads(t, name, device, dtype=None, rows=None):
-    """[rows, heads, d] with contiguous dims; any row and head strides."""
-    if t.dim() != 3 or t.device != device or t.dtype not in _TYPES or (dtype is not None and t.dtype != dtype) or (
-            rows is not None and t.shape[0] != rows) or (t.shape[2] > 1 and t.stride(2) != 1):
-        raise ValueError(f"{name} must be a [rows, heads, d] tensor on {device} with contiguous dims"
-                         + (f" of type {dtype}" if dtype is not None else ""))
-    return t.data_ptr()
+def _strides(t, name, device, shape, types):
+    """(address, row stride, head stride) of a [rows, heads, d] tensor with
+    contiguous dims and any row and head strides."""
+    if t.shape != shape or t.dtype not in types or t.device != device:
+        raise ValueError(f"{name} must be a {list(shape)} tensor on {device}, of " + " or ".join(map(str, types)))
+    row, head, one = t.stride()
+    if one != 1:
+        raise ValueError(f"{name} must have contiguous dims")
+    return t.data_ptr(), row, head
+
+
+def _pool_heads(pool):
+    """(kv heads, dims) that a pool holds."""
+    if pool.dim() != 3 or pool.shape[2] % 18:
+        raise ValueError("pool must be uint8 [num_blocks, n_kv, 18 * d_head] (see new_kv4_pool)")
+    return pool.shape[1], pool.shape[2] // 18
 
 
 def kv4_append(pool, k, v, pos, table, *, seq=None, q=None, q_out=None, cos=None, sin=None, interleaved=False,
@@ -92,42 +111,44 @@ def kv4_append(pool, k, v, pos, table, *, seq=None, q=None, q_out=None, cos=None
     rotation.  ``q`` [n, heads, d] is turned alike into ``q_out`` (default: a
     new tensor; may be ``q``; a float32 ``q`` also into bf16 or fp16), which is
     returned.  Two rows at one position: the cache gets dims of either."""
-    d = k.shape[-1] if k.dim() == 3 else 0
-    c = _cache(pool, table, status, k.shape[1] if k.dim() == 3 else 0, d)
-    dev, n = pool.device, k.shape[0]
-    r = _lib.Kv4Rows(k=_heads(k, "k", dev), v=_heads(v, "v", dev, k.dtype, n), dtype=_TYPES[k.dtype], n_rows=n,
-                     k_row=k.stride(0), k_head=k.stride(1), v_row=v.stride(0), v_head=v.stride(1))
-    if v.shape != k.shape:
-        raise ValueError("v must have k's shape")
-    r.pos = _ints(pos, "pos", dev, n)
-    if seq is not None:
-        r.seq = _ints(seq, "seq", dev, n)
-    elif n > table.shape[0]:
+    n_kv, d = _pool_heads(pool)
+    c = _cache(pool, table, status, n_kv, d)
+    dev, n = pool.device, pos.numel()
+    shape = (n, n_kv, d)
+    k_ptr, k_row, k_head = _strides(k, "k", dev, shape, _TYPES)
+    v_ptr, v_row, v_head = _strides(v, "v", dev, shape, (k.dtype,))
+    if seq is None and n > table.shape[0]:
         raise ValueError("more rows than table rows need seq")
+    heads = rotary = max_pos = q_row = q_head = o_row = o_head = 0
+    q_ptr = o_ptr = None
+    dtype = o_type = _TYPES[k.dtype]
     if q is not None:
-        r.q = _heads(q, "q", dev, k.dtype, n)
-        if q.shape[2] != d or q.shape[1] < 1:
-            raise ValueError("q must have heads of k's dims")
+        heads = q.shape[1] if q.dim() == 3 else 0
+        q_ptr, q_row, q_head = _strides(q, "q", dev, (n, heads, d), (k.dtype,))
+        if heads < 1:
+            raise ValueError("q needs a head")
         if q_out is None:
-            with torch.cuda.stream(stream or torch.cuda.current_stream(dev)):
-                q_out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-        r.q_out = _heads(q_out, "q_out", dev, None if q.dtype == torch.float32 else q.dtype, n)
-        if q_out.shape != q.shape or (q_out.data_ptr() == q.data_ptr() and
-                                      (q_out.stride() != q.stride() or q_out.dtype != q.dtype)):
-            raise ValueError("q_out must have q's shape (and be q or apart from it)")
-        r.q_row, r.q_head, r.q_out_row, r.q_out_head = q.stride(0), q.stride(1), q_out.stride(0), q_out.stride(1)
-        r.n_heads, r.q_out_dtype = q.shape[1], _TYPES[q_out.dtype]
+            q_out = _empty(q.shape, q.dtype, dev, stream)
+        o_ptr, o_row, o_head = _strides(q_out, "q_out", dev, q.shape,
+                                        _TYPES if q.dtype == torch.float32 else (q.dtype,))
+        o_type = _TYPES[q_out.dtype]
+        if o_ptr == q_ptr and n and (q_out.stride() != q.stride() or o_type != dtype):
+            raise ValueError("q_out must be q or apart from it")
     elif q_out is not None:
         raise ValueError("q_out without q")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin go together")
     if cos is not None:
-        for t, name in ((cos, "cos"), (sin, "sin")):
-            if t.dtype != torch.float32 or t.device != dev or t.dim() != 2 or not t.is_contiguous() or (
-                    t.shape != cos.shape) or not 1 <= 2 * t.shape[1] <= d or t.shape[0] < 1:
-                raise ValueError(f"{name} must be contiguous float32 [max_pos, r / 2] with 2 <= r <= {d} on {dev}")
-        r.cos, r.sin, r.rotary_dim, r.max_pos = cos.data_ptr(), sin.data_ptr(), 2 * cos.shape[1], cos.shape[0]
-        r.interleaved = int(bool(interleaved))
+        max_pos, half = cos.shape if cos.dim() == 2 else (0, 0)
+        rotary = 2 * half
+        for t in (cos, sin):
+            if t.dtype != torch.float32 or t.shape != (max_pos, half) or t.device != dev or not t.is_contiguous() or (
+                    not 2 <= rotary <= d) or max_pos < 1:
+                raise ValueError(f"cos and sin must be contiguous float32 [max_pos, r / 2] on {dev}, 2 <= r <= {d}")
+    r = _lib.Kv4Rows(q_ptr, k_ptr, v_ptr, o_ptr, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head,
+                     _ints(pos, "pos", dev, n), None if seq is None else _ints(seq, "seq", dev, n),
+                     None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), dtype, o_type, n,
+                     heads, rotary, 1 if interleaved else 0, max_pos)
     if n:
         _lib.check(_lib.load().b2d_kv4_append(ctypes.byref(c), ctypes.byref(r), _stream_on(stream, dev)),
                    "b2d_kv4_append")
@@ -138,20 +159,22 @@ def kv4_read(pool, pos, table, *, seq=None, dtype=torch.bfloat16, status=None, s
     """The rows at positions ``pos`` of the sequences ``seq`` (as in
     ``kv4_append``) as values: ``(k, v)``, each [n, n_kv, d] of ``dtype``
     (float32, bf16 or fp16, all exact); zeros where ``pos`` is negative."""
-    n_kv, d = (pool.shape[1], pool.shape[2] // 18) if pool.dim() == 3 else (0, 0)
+    n_kv, d = _pool_heads(pool)
     c = _cache(pool, table, status, n_kv, d)
     dev, n = pool.device, pos.numel()
     if dtype not in _TYPES:
         raise ValueError("dtype must be float32, bfloat16 or float16")
     if seq is None and n > table.shape[0]:
         raise ValueError("more rows than table rows need seq")
-    p, s = _ints(pos, "pos", dev, n), _ints(seq, "seq", dev, n) if seq is not None else None
-    with torch.cuda.stream(stream or torch.cuda.current_stream(dev)):
-        k, v = (torch.empty(n, n_kv, d, dtype=dtype, device=dev) for _ in range(2))
+    p, s = _ints(pos, "pos", dev, n), None if seq is None else _ints(seq, "seq", dev, n)
+    k, v = (_empty((n, n_kv, d), dtype, dev, stream) for _ in range(2))
     if n:
         _lib.check(_lib.load().b2d_kv4_read(ctypes.byref(c), p, s, n, _TYPES[dtype], k.data_ptr(), v.data_ptr(),
                                             _stream_on(stream, dev)), "b2d_kv4_read")
     return k, v
+
+
+_QUERY_TYPES = (torch.bfloat16, torch.float16)
 
 
 def kv4_attention(q, pool, lens, table, *, q_start=None, max_rows=None, max_len=None, scale=None, out=None,
@@ -166,48 +189,48 @@ def kv4_attention(q, pool, lens, table, *, q_start=None, max_rows=None, max_len=
     ``max_rows`` (default: n), and rows of no sequence stay as they are.
     ``max_len`` (default: what a table row holds) bounds ``lens``; a close
     bound splits long sequences better.  ``scale`` defaults to d ** -0.5."""
-    n_kv, d = (pool.shape[1], pool.shape[2] // 18) if pool.dim() == 3 else (0, 0)
+    n_kv, d = _pool_heads(pool)
     c = _cache(pool, table, status, n_kv, d)
     dev = pool.device
-    _heads(q, "q", dev)
-    n, heads = q.shape[:2]
-    if q.dtype not in (torch.bfloat16, torch.float16) or q.shape[2] != d or heads < 1 or heads % n_kv:
-        raise ValueError(f"q must be bf16 or fp16 [rows, a multiple of {n_kv} heads, {d}]")
-    n_seqs = lens.numel()
-    if n_seqs > table.shape[0]:
+    n, heads = q.shape[:2] if q.dim() == 3 else (0, 0)
+    q_ptr, q_row, q_head = _strides(q, "q", dev, (n, heads, d), _QUERY_TYPES)
+    if heads < 1 or heads % n_kv:
+        raise ValueError(f"q must have a multiple of {n_kv} heads")
+    n_seqs, (rows, bps) = lens.numel(), table.shape
+    if n_seqs > rows:
         raise ValueError("more lengths than table rows")
-    if q_start is None and n_seqs != n:
-        raise ValueError("without q_start there is one row a sequence")
     if out is None:
-        with torch.cuda.stream(stream or torch.cuda.current_stream(dev)):
-            out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    _heads(out, "out", dev, q.dtype, n)
-    if out.shape != q.shape:
-        raise ValueError("out must have q's shape")
-    room = min(table.shape[1] * PAGE_TOKENS, 2 ** 31 - 1)
+        out = _empty(q.shape, q.dtype, dev, stream)
+    o_ptr, o_row, o_head = _strides(out, "out", dev, q.shape, (q.dtype,))
+    room = min(bps * PAGE_TOKENS, 2 ** 31 - 1)
     max_len = room if max_len is None else int(max_len)
-    max_rows = (1 if q_start is None else max(1, n)) if max_rows is None else int(max_rows)
     if not 0 <= max_len <= room:
         raise ValueError(f"max_len must be in [0, {room}] (the table's rows)")
-    if max_rows < 1 or (q_start is None and max_rows != 1):
-        raise ValueError("max_rows must be at least 1, and 1 without q_start")
+    lens_ptr, start_ptr = _ints(lens, "lens", dev, n_seqs), None
+    if q_start is None:
+        if n_seqs != n or max_rows not in (None, 1):
+            raise ValueError("without q_start there is one row a sequence")
+        max_rows = 1
+    else:
+        start_ptr = _ints(q_start, "q_start", dev, n_seqs + 1)
+        max_rows = max(1, n) if max_rows is None else int(max_rows)
+        if max_rows < 1:
+            raise ValueError("max_rows must be at least 1")
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError("scale must be positive")
-    query = _lib.Kv4Query(q.data_ptr(), out.data_ptr(), q.stride(0), q.stride(1), out.stride(0), out.stride(1),
-                          _ints(lens, "lens", dev, n_seqs),
-                          _ints(q_start, "q_start", dev, n_seqs + 1) if q_start is not None else None,
-                          _TYPES[q.dtype], n, heads, n_seqs, max_rows, max_len, scale)
     if not n or not n_seqs:
         return out
-    lib, need = _lib.load(), ctypes.c_uint64()
+    lib, stream_ptr = _lib.load(), _stream_on(stream, dev)
+    query = _lib.Kv4Query(q_ptr, o_ptr, q_row, q_head, o_row, o_head, lens_ptr, start_ptr, _TYPES[q.dtype], n, heads,
+                          n_seqs, max_rows, max_len, scale)
+    need = ctypes.c_uint64()
     _lib.check(lib.b2d_kv4_attention_scratch(ctypes.byref(c), ctypes.byref(query), ctypes.byref(need)),
                "b2d_kv4_attention_scratch")
     scratch = None
     if need.value:  # from the stream's own memory: calls on other streams, and other graphs, have theirs
-        with torch.cuda.stream(stream or torch.cuda.current_stream(dev)):
-            scratch = torch.empty(need.value, dtype=torch.uint8, device=dev)
+        scratch = _empty(need.value, torch.uint8, dev, stream)
     _lib.check(lib.b2d_kv4_attention(ctypes.byref(c), ctypes.byref(query),
-                                     scratch.data_ptr() if scratch is not None else None, need.value,
-                                     _stream_on(stream, dev)), "b2d_kv4_attention")
+                                     None if scratch is None else scratch.data_ptr(), need.value, stream_ptr),
+               "b2d_kv4_attention")
     return out
