@@ -87,7 +87,7 @@ def attention_bound(out, mass, size, length, d, half_step, vmax):
     """How far the kernel may be off.  ``half_step``: finfo(type).eps / 2.
 
     * the result is rounded once: half_step |o|;
-    * each probability is rounded to the type: half_step of sum p |v|;
+    * each probability is rounded to a half: 2^-11 of sum p |v|;
     * a score is a float32 sum of d products, scaled once, minus the maximum:
       off by (d + 3) 2^-24 of sum |q k|, which shifts log2 p by that times
       log2(e); with the maximum's own, p changes by twice that share, and so
@@ -97,12 +97,12 @@ def attention_bound(out, mass, size, length, d, half_step, vmax):
     * float32 sums over the positions: a chain of length / 16 products of 16
       and the rescaling after each, (length / 16 + 64) 2^-23 of sum p |v|,
       again for numerator and divisor;
-    * fp16 alone, whose numbers below 2^-14 are 2^-24 apart: the result's
-      rounding is off by up to 2^-25 however small it is, and a probability,
-      held with a factor of 2^15 that the row's sum (at least that factor)
-      carries too, by up to 2^-25 / 2^15 = 2^-40, at each of `length` positions
-      with |v| <= vmax.
+    * a probability is a half with a factor of 2^15 that the row's sum (at least
+      that factor) carries too; halves below 2^-14 are 2^-24 apart, so it is off
+      by up to 2^-25 / 2^15 = 2^-40, at each of `length` positions with
+      |v| <= vmax;
+    * an fp16 result's rounding is off by up to 2^-25 however small it is.
     """
-    low = 2.0 ** -25 + length * 2.0 ** -40 * vmax if half_step == 2.0 ** -11 else 0.0
-    share = half_step + 4 * (d + 6) * 2.0 ** -24 * size + 2.0 ** -20 + 2 * (length / 16 + 64) * 2.0 ** -23
+    low = length * 2.0 ** -40 * vmax + (2.0 ** -25 if half_step == 2.0 ** -11 else 0.0)
+    share = 2.0 ** -11 + 4 * (d + 6) * 2.0 ** -24 * size + 2.0 ** -20 + 2 * (length / 16 + 64) * 2.0 ** -23
     return half_step * np.abs(out) + share * (1 + half_step) * mass + low + 1e-30

@@ -1,7 +1,10 @@
 // kv4.cu — launches of the 4-bit KV cache's kernels and their C entry points
 // (b2d_kv4_* in include/b2d.h).
 #include <algorithm>
+#include <atomic>
 #include <cmath>
+#include <cstdlib>
+#include <cstdlib>
 #include <cstring>
 
 #include "b2d_host.h"
@@ -21,22 +24,45 @@ cudaError_t append_typed(const Kv4AppendArgs& a, cudaStream_t st, bool pdl) {
   return launch(kv4_append_kernel<T, TQ>, grid, dim3(kKv4AppendThreads), 0, st, pdl, a, heads);
 }
 
-template <class Op, int NH, int NB>
-cudaError_t attn_shape(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
-  const int64_t units = static_cast<int64_t>(a.n_seqs) * a.c.n_kv * a.tiles;
-  cudaError_t e = launch(kv4_attn_kernel<Op, NH, NB>, dim3(static_cast<unsigned>(units * a.splits)),
-                         dim3(32 * kKv4Warps), 0, st, pdl, a);
-  if (e == cudaSuccess && a.splits > 1)
-    e = launch(kv4_join_kernel<Op, NH, NB>, dim3(static_cast<unsigned>((units * 8 * NB + 7) / 8)), dim3(256), 0, st,
-               true, a);
+// Dynamic shared memory past 48 KB is granted per kernel and device, once.
+template <auto Kernel, int Bytes>
+cudaError_t raise_smem() {
+  if (Bytes <= 48 * 1024) return cudaSuccess;
+  static std::atomic<bool> raised[64];
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev < 64 && raised[dev].load(std::memory_order_relaxed)) return cudaSuccess;
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Bytes);
+  if (e == cudaSuccess && dev < 64) raised[dev].store(true, std::memory_order_relaxed);
   return e;
 }
 
-template <class Op>
+template <class T, int NH, int NB, int W>
+cudaError_t attn_launch(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
+  constexpr int smem = kv4_attn_smem<NH, NB, W>();
+  cudaError_t e = raise_smem<kv4_attn_kernel<T, NH, NB, W>, smem>();
+  const unsigned x = static_cast<unsigned>(a.n_seqs), y = static_cast<unsigned>(a.c.n_kv);
+  if (e == cudaSuccess)
+    e = launch(kv4_attn_kernel<T, NH, NB, W>, dim3(x, y, static_cast<unsigned>(a.tiles * a.splits)), dim3(32 * W), smem,
+               st, pdl, a);
+  if (e == cudaSuccess && a.splits > 1)
+    e = launch(kv4_join_kernel<T, NH>, dim3(x, y, static_cast<unsigned>(a.max_rows * a.group)), dim3(128), 0, st, true,
+               a);
+  return e;
+}
+
+template <class T, int NH>
+cudaError_t attn_shape(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
+  if (a.tile_cols > 8) return attn_launch<T, NH, 2, 4>(a, st, pdl);
+  if (a.warps == 1) return attn_launch<T, NH, 1, 1>(a, st, pdl);
+  if (a.warps == 2) return attn_launch<T, NH, 1, 2>(a, st, pdl);
+  return attn_launch<T, NH, 1, 4>(a, st, pdl);
+}
+
+template <class T>
 cudaError_t attn_typed(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
-  const bool wide = a.tile_cols > 8;
-  if (a.c.d == 64) return wide ? attn_shape<Op, 1, 2>(a, st, pdl) : attn_shape<Op, 1, 1>(a, st, pdl);
-  return wide ? attn_shape<Op, 2, 2>(a, st, pdl) : attn_shape<Op, 2, 1>(a, st, pdl);
+  return a.c.d == 64 ? attn_shape<T, 1>(a, st, pdl) : attn_shape<T, 2>(a, st, pdl);
 }
 
 }  // namespace
@@ -61,17 +87,27 @@ cudaError_t kv4_read(const Kv4ReadArgs& a, cudaStream_t st) {
   return launch(kv4_read_kernel<__nv_bfloat16>, grid, block, 0, st, false, a);
 }
 
-void kv4_attn_plan(Kv4AttnArgs& a, int sms) {
-  const int64_t cols = static_cast<int64_t>(a.max_rows) * (a.n_heads / a.c.n_kv);
+bool kv4_attn_plan(Kv4AttnArgs& a, int sms) {
+  a.group = a.n_heads / a.c.n_kv;
+  a.group_inv = ((uint64_t(1) << 32) + a.group - 1) / a.group;
+  const int64_t cols = static_cast<int64_t>(a.max_rows) * a.group;
+  if (cols * a.group >= int64_t(1) << 32) return false;
   a.tile_cols = cols <= 8 ? 8 : 16;
   a.tiles = static_cast<int>((cols + a.tile_cols - 1) / a.tile_cols);
   const int pages = std::max(1, (a.max_len + kKv4Page - 1) / kKv4Page);
   const int64_t units = static_cast<int64_t>(a.n_seqs) * a.c.n_kv * a.tiles;
-  // enough CTAs for the GPU, at least 8 pages (two a warp) each
-  const int64_t want = std::max<int64_t>(1, int64_t(sms) * 4 / std::max<int64_t>(1, units));
-  const int64_t splits = std::min<int64_t>(want, std::max(1, pages / 8));
+  // Splits: at least 32 pages each (8 a warp).  One sequence's splits are alike:
+  // one wave of CTAs, four to an SM (131071 positions, 8 kv heads of 128: 45 us,
+  // and 55 us with splits for four waves).  Several sequences differ in length:
+  // four waves even that out (32 of 1001 to 16384: 93 us, and 110 us with one).
+  const int64_t ctas = int64_t(sms) * (a.n_seqs == 1 ? 4 : 16);
+  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(ctas / std::max<int64_t>(1, units), (pages + 31) / 32));
   a.split_pages = static_cast<int>((pages + splits - 1) / splits);
   a.splits = (pages + a.split_pages - 1) / a.split_pages;
+  a.warps = 4;
+  if (getenv("KV4_W")) a.warps = atoi(getenv("KV4_W"));
+  // the grid's y and z
+  return a.c.n_kv <= 65535 && int64_t(a.tiles) * a.splits <= 65535 && (a.splits == 1 || cols <= 65535);
 }
 
 uint64_t kv4_attn_scratch(const Kv4AttnArgs& a) {
@@ -81,7 +117,7 @@ uint64_t kv4_attn_scratch(const Kv4AttnArgs& a) {
 
 cudaError_t kv4_attention(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
   if (a.n_rows == 0 || a.n_seqs == 0) return cudaSuccess;
-  return a.dtype == B2D_F16 ? attn_typed<Kv4Half>(a, st, pdl) : attn_typed<Kv4Bf16>(a, st, pdl);
+  return a.dtype == B2D_F16 ? attn_typed<__half>(a, st, pdl) : attn_typed<__nv_bfloat16>(a, st, pdl);
 }
 
 }  // namespace b2d
@@ -140,9 +176,7 @@ b2d_status check_query(const b2d_kv4_cache* c, const b2d_kv4_query* q, b2d::Kv4A
   int sms = 0;
   const cudaError_t e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, c->device);
   if (e != cudaSuccess) return b2d::cuda_failed(e, "SM count");
-  b2d::kv4_attn_plan(a, sms);
-  if (int64_t(a.n_seqs) * a.c.n_kv * a.tiles * a.splits > kMaxBlocks) return B2D_ERR_UNSUPPORTED;
-  return B2D_OK;
+  return b2d::kv4_attn_plan(a, sms) ? B2D_OK : B2D_ERR_UNSUPPORTED;
 }
 
 }  // namespace

@@ -49,7 +49,7 @@ __device__ __forceinline__ float kv4_scale_value(uint32_t byte) {
 __device__ __forceinline__ void kv4_error(uint32_t* status, uint32_t code) {
   if (status != nullptr) atomicCAS(status, 0u, code);
 }
-constexpr uint32_t kKv4BadPos = 0x202u, kKv4BadTable = 0x203u;
+constexpr uint32_t kKv4BadPos = 0x202u, kKv4BadTable = 0x203u, kKv4Timeout = 0x10Du;
 
 // The page of position `pos` of the sequence with table row `sid`, or null
 // (status set) when the table does not name one.
@@ -349,70 +349,125 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ K
 }
 
 // ---- attention -----------------------------------------------------------------------
-// S^T = K Q^T and O^T = V^T P^T on m16n8k16: the 16 positions of a page are
-// the rows of the first product and the reduction of the second, the query
+// S^T = K Q^T and O^T = V^T P^T on m16n8k16 in half: the 16 positions of a page
+// are the rows of the first product and the reduction of the second, the query
 // columns (row of the sequence, head of the group) its 8 columns, so no
-// fragment of the cache is wasted on absent queries.  The held values are
-// exact in the operands' type: a nibble becomes 128 + u (bf16) or 1024 + u
-// (half) by one logic instruction, and value = scale * (u - 8).
+// fragment of the cache is wasted on absent queries.
+//
+// Both operands of both products are exact but for the probabilities: held
+// values are halves, half queries are taken as they are, and bf16 queries (8
+// significant bits) become halves after each column is divided by the power of
+// two below its largest magnitude, which the softmax scale takes back; what
+// that loses of dims 2^28 times smaller than the largest is far below a
+// float32 sum's own rounding.  Probabilities keep 11 bits: they carry a factor
+// 2^15, so those down to 2^-29 of the row's largest are normal halves, and the
+// sum they are divided by carries it too.
+constexpr float kKv4POffset = 15.f;
 
-// Operands in bf16: value = (128 + u) s - 136 s, one fma, exact: 136 s has at
-// most 8 significant bits and the result at most 7.
-struct Kv4Bf16 {
-  using T = __nv_bfloat16;
-  static constexpr float kPOffset = 0.f;
-  // scale pair from the bytes b0 << 8 | b1 << 24: the byte's bits as a bf16 with a
-  // tiny exponent (subnormal for b < 8), times 2^112
-  static __device__ __forceinline__ uint32_t scale(uint32_t bytes) {
-    uint32_t s;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(s) : "r"(bytes >> 4), "r"(0x77807780u));
-    return s;
+// Four halves-pairs of a code word: nibbles (i, i + 4) for i = 0 .. 3, each
+// times its scale.  1024 + u (bits 0-3 of a half's mantissa) less 1032, or
+// 1024 + 16 u (bits 4-7) over 16 less 72, is u - 8 exactly; so is the product.
+__device__ __forceinline__ void kv4_values(uint32_t w, uint32_t s, uint32_t (&v)[4]) {
+  const uint32_t x = w >> 8;
+  asm("{\n\t.reg .b32 a, b, c, d;\n\t"
+      "lop3.b32 a, %4, 0x000F000F, 0x64006400, 0xEA;\n\t"
+      "lop3.b32 b, %4, 0x00F000F0, 0x64006400, 0xEA;\n\t"
+      "lop3.b32 c, %5, 0x000F000F, 0x64006400, 0xEA;\n\t"
+      "lop3.b32 d, %5, 0x00F000F0, 0x64006400, 0xEA;\n\t"
+      "sub.rn.f16x2 a, a, %7;\n\t"
+      "fma.rn.f16x2 b, b, %8, %9;\n\t"
+      "sub.rn.f16x2 c, c, %7;\n\t"
+      "fma.rn.f16x2 d, d, %8, %9;\n\t"
+      "mul.rn.f16x2 %0, a, %6;\n\t"
+      "mul.rn.f16x2 %1, b, %6;\n\t"
+      "mul.rn.f16x2 %2, c, %6;\n\t"
+      "mul.rn.f16x2 %3, d, %6;\n\t}"
+      : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+      : "r"(w), "r"(x), "r"(s), "r"(0x64086408u), "r"(0x2C002C00u), "r"(0xD480D480u));
+}
+// Scale pair from two bytes of w: selector 0x4i4j puts bytes j, i into the halves.
+__device__ __forceinline__ uint32_t kv4_scales(uint32_t w, uint32_t selector) {
+  return __byte_perm(w, 0u, selector) * 128u;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+__device__ __forceinline__ void mma_half(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_half_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {  // d = a b
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+// A column's query fragments: f[h][2 s], f[h][2 s + 1] for k-step s, dims (s, s + 4)
+// and (8 + s, 12 + s) of the lane's 16 at q + 64 h.  Returns the power of two the
+// column was divided by (the four lanes of a column agree on it).
+template <class T>
+__device__ __forceinline__ void load16(const T* p, uint32_t (&w)[8], bool in, bool vec) {  // 16 elements of 2 bytes
+  if (!in) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = 0u;
+  } else if (vec) {
+    const uint4 x = *reinterpret_cast<const uint4*>(p), y = *reinterpret_cast<const uint4*>(p + 8);
+    w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+    w[4] = y.x; w[5] = y.y; w[6] = y.z; w[7] = y.w;
+  } else {
+    const uint16_t* b = reinterpret_cast<const uint16_t*>(p);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) w[i] = b[2 * i] | (static_cast<uint32_t>(b[2 * i + 1]) << 16);
   }
-  static __device__ __forceinline__ uint32_t offset(uint32_t s) {
-    uint32_t c;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(c) : "r"(s), "r"(0xC308C308u));  // -136
-    return c;
+}
+template <int NH>
+__device__ __forceinline__ float kv4_query(const __half* q, bool in, bool vec, uint32_t (&f)[NH][8]) {
+#pragma unroll
+  for (int h = 0; h < NH; ++h) {
+    uint32_t w[8];
+    load16(q + 64 * h, w, in, vec);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      const uint32_t sel = s & 1 ? 0x7632 : 0x5410;  // the odd or even elements of two words
+      f[h][2 * s] = __byte_perm(w[s >> 1], w[2 + (s >> 1)], sel);
+      f[h][2 * s + 1] = __byte_perm(w[4 + (s >> 1)], w[6 + (s >> 1)], sel);
+    }
   }
-  static __device__ __forceinline__ uint32_t value(uint32_t w, uint32_t s, uint32_t c) {
-    uint32_t v;
-    asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(v) : "r"((w & 0x000F000Fu) | 0x43004300u), "r"(s), "r"(c));
-    return v;
+  return 1.f;
+}
+template <int NH>
+__device__ __forceinline__ float kv4_query(const __nv_bfloat16* q, bool in, bool vec, uint32_t (&f)[NH][8]) {
+  uint32_t w[NH][8], top = 0;
+#pragma unroll
+  for (int h = 0; h < NH; ++h) {
+    load16(q + 64 * h, w[h], in, vec);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t x = w[h][i] & 0x7F807F80u;  // both exponents, the upper one leading
+      top = max(top, max(x, x << 16));
+    }
   }
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    mma_bf16(d, a[0], a[1], a[2], a[3], b0, b1);
-  }
-};
-// Operands in half: 1032 s may exceed the type, so the offset goes first:
-// (1024 + u) - 1032, then times s, both exact.
-// Probabilities carry a factor 2^15, so that those down to 2^-29 of the row's
-// largest keep 11 bits; the sum carries it too.
-struct Kv4Half {
-  using T = __half;
-  static constexpr float kPOffset = 15.f;
-  static __device__ __forceinline__ uint32_t scale(uint32_t bytes) { return bytes >> 1; }
-  static __device__ __forceinline__ uint32_t offset(uint32_t) { return 0u; }
-  static __device__ __forceinline__ uint32_t value(uint32_t w, uint32_t s, uint32_t) {
-    uint32_t v;
-    asm("{\n\t.reg .b32 u;\n\tsub.rn.f16x2 u, %1, %2;\n\tmul.rn.f16x2 %0, u, %3;\n\t}"
-        : "=r"(v) : "r"((w & 0x000F000Fu) | 0x64006400u), "r"(0x64086408u), "r"(s));
-    return v;
-  }
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __half2 v = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t*>(&v);
-  }
-  static __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
-        "{%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-};
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2)) >> 23;
+  const int e = top == 0 ? 0 : min(static_cast<int>(top), 253) - 127;
+  const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
+#pragma unroll
+  for (int h = 0; h < NH; ++h)
+#pragma unroll
+    for (int s = 0; s < 4; ++s)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t x = w[h][4 * k + (s >> 1)], y = w[h][4 * k + 2 + (s >> 1)];
+        f[h][2 * s + k] = s & 1 ? pack_half2(bf16_hi(x) * down, bf16_hi(y) * down)
+                                : pack_half2(bf16_lo(x) * down, bf16_lo(y) * down);
+      }
+  return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
 
 __device__ __forceinline__ float exp2_fast(float x) {  // 2^x (2 ulp), 0 at -infinity
   float y;
@@ -425,36 +480,40 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-constexpr int kKv4Warps = 4;
-
-// Where a tile's work lies: sequence, kv head, tile of query columns, split.
+// Where a CTA's work lies.  Grid: x = sequence, y = kv head, z = tile of query
+// columns + tiles * split.
 struct Kv4Tile {
   int seq, g, tile, split;
-  int r0, rows, len, group;
-  __device__ __forceinline__ int cols() const { return rows * group; }
-  // positions that column c sees
-  __device__ __forceinline__ int limit(int c) const { return min(len, max(0, len - rows + c / group + 1)); }
+  int r0, rows, len;
+  __device__ __forceinline__ int cols(const Kv4AttnArgs& a) const { return rows * a.group; }
 };
-
+__device__ __forceinline__ int kv4_row(const Kv4AttnArgs& a, int col) {  // col / group
+  return static_cast<int>(static_cast<uint64_t>(static_cast<uint32_t>(col)) * a.group_inv >> 32);
+}
+// positions that column c sees
+__device__ __forceinline__ int kv4_limit(const Kv4AttnArgs& a, const Kv4Tile& t, int c) {
+  return t.rows == 1 ? t.len : min(t.len, max(0, t.len - t.rows + kv4_row(a, c) + 1));
+}
 // False when the tile has no columns.  Bad inputs (lengths past the table or
 // max_len, rows past n_rows or max_rows) leave rows or len 0 and set the status.
-__device__ __forceinline__ bool kv4_tile(const Kv4AttnArgs& a, int u, int cols_per_tile, Kv4Tile& t) {
-  t.tile = u % a.tiles;
-  u /= a.tiles;
-  t.split = u % a.splits;
-  u /= a.splits;
-  t.g = u % a.c.n_kv;
-  t.seq = u / a.c.n_kv;
-  t.group = a.n_heads / a.c.n_kv;
-  t.r0 = a.q_start != nullptr ? a.q_start[t.seq] : t.seq;
-  t.rows = a.q_start != nullptr ? a.q_start[t.seq + 1] - t.r0 : 1;
-  if (t.rows <= 0) return false;
-  if (t.r0 < 0 || t.rows > a.max_rows || t.rows > a.n_rows - t.r0) {
-    if (threadIdx.x == 0) kv4_error(a.c.status, kKv4BadPos);
-    return false;
+__device__ __forceinline__ bool kv4_tile(const Kv4AttnArgs& a, int z, Kv4Tile& t) {
+  t.seq = blockIdx.x;
+  t.g = blockIdx.y;
+  t.split = a.tiles == 1 ? z : z / a.tiles;
+  t.tile = z - t.split * a.tiles;
+  t.len = __ldg(a.lens + t.seq) + a.len_add;
+  t.r0 = t.seq;
+  t.rows = 1;
+  if (a.q_start != nullptr) {
+    t.r0 = __ldg(a.q_start + t.seq);
+    t.rows = __ldg(a.q_start + t.seq + 1) - t.r0;
+    if (t.rows <= 0) return false;
+    if (t.r0 < 0 || t.rows > a.max_rows || t.rows > a.n_rows - t.r0) {
+      if (threadIdx.x == 0) kv4_error(a.c.status, kKv4BadPos);
+      return false;
+    }
+    if (t.tile * a.tile_cols >= t.cols(a)) return false;
   }
-  if (t.tile * cols_per_tile >= t.cols()) return false;
-  t.len = a.lens[t.seq] + a.len_add;
   if (t.len > a.max_len) {
     if (threadIdx.x == 0) kv4_error(a.c.status, kKv4BadPos);
     t.len = 0;
@@ -462,60 +521,121 @@ __device__ __forceinline__ bool kv4_tile(const Kv4AttnArgs& a, int u, int cols_p
   if (t.len < 0) t.len = 0;
   return true;
 }
-// Pages that a tile's columns see, and the splits that have some of them.
-__device__ __forceinline__ int kv4_tile_pages(const Kv4Tile& t, int cols_per_tile) {
-  const int last = min(t.cols(), (t.tile + 1) * cols_per_tile) - 1;
-  return (t.limit(last) + kKv4Page - 1) / kKv4Page;
+// Pages that a tile's columns see.
+__device__ __forceinline__ int kv4_tile_pages(const Kv4AttnArgs& a, const Kv4Tile& t) {
+  const int last = min(t.cols(a), (t.tile + 1) * a.tile_cols) - 1;
+  return (kv4_limit(a, t, last) + kKv4Page - 1) / kKv4Page;
 }
 
-// One CTA of 4 warps per (sequence, kv head, tile of 8 NB query columns, split
-// of the positions).  Warp w takes the split's pages w, w + 4, ...; each runs
-// its own online softmax, and the four meet in shared memory at the end.
-template <class Op, int NH, int NB>
-__global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
-  using T = typename Op::T;
-  constexpr int D = 64 * NH, COLS = 8 * NB;
-  __shared__ float s_o[kKv4Warps][COLS][D];
-  __shared__ float s_m[kKv4Warps][COLS], s_l[kKv4Warps][COLS];
+// A split's share of a column: d floats of o, then its maximum and sum.
+__device__ __forceinline__ float* kv4_part(const Kv4AttnArgs& a, int seq, int g, int tile, int split, int col, int d) {
+  const int64_t unit = (static_cast<int64_t>(seq) * a.c.n_kv + g) * a.tiles + tile;
+  return a.part + ((unit * a.splits + split) * a.tile_cols + col) * (d + 4);
+}
+
+// The pages of a warp's ring: kKv4Ahead + 1 steps of P pages.
+constexpr int kKv4Ahead = 2;
+constexpr uint64_t kKv4WaitNs = 200000000ull;  // bound on every page wait
+constexpr __host__ __device__ int kv4_step_pages(int nh) { return nh == 1 ? 4 : 2; }
+template <int NH, int NB, int W>
+constexpr __host__ __device__ int kv4_attn_smem() {
+  constexpr int ring = W * (kKv4Ahead + 1) * kv4_step_pages(NH) * kv4_page_bytes(64 * NH);
+  constexpr int join = W == 1 ? 0 : W * 8 * NB * (64 * NH + 2) * 4;  // reuses the ring
+  return ring > join ? ring : join;
+}
+
+// One CTA of W warps per (sequence, kv head, tile of 8 NB query columns, split
+// of the positions).  Warp w takes the split's pages w, w + W, ...; each runs
+// its own online softmax, and the warps meet in shared memory at the end.
+// A page's bytes are contiguous: each comes by one bulk copy into the warp's
+// ring, kKv4Ahead steps ahead; a step takes P pages, so the running maximum
+// and the rescaling of o are paid once for 16 P positions.
+template <class T, int NH, int NB, int W>
+__global__ void __launch_bounds__(32 * W) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
+  constexpr int D = 64 * NH, COLS = 8 * NB, P = kv4_step_pages(NH), PB = kv4_page_bytes(D), SLOTS = kKv4Ahead + 1;
+  extern __shared__ __align__(16) uint8_t kv4_smem[];
+  __shared__ uint64_t s_bar[W][SLOTS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
+  uint64_t* bar = s_bar[warp];
+  if (lane == 0) {
+    for (int i = 0; i < SLOTS; ++i) mbar_init(&bar[i], 1);
+    fence_mbar_init();
+  }
+  __syncwarp();
   pdl_wait();
   pdl_launch();
   Kv4Tile tl;
-  if (!kv4_tile(a, blockIdx.x, COLS, tl)) return;
-  const int pages = kv4_tile_pages(tl, COLS);
+  if (!kv4_tile(a, blockIdx.z, tl)) return;
+  const int pages = kv4_tile_pages(a, tl);
   const int lo = tl.split * a.split_pages, hi = min(pages, lo + a.split_pages);
   if (lo >= hi && tl.split > 0) return;  // (the first split always answers)
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
-  const int c0 = tl.tile * COLS, cols = tl.cols();
+  const int c0 = tl.tile * COLS, cols = tl.cols(a);
+
+  // ---- the warp's pages: the k-th is lo + warp + W k ----
+  const int32_t* table = a.c.table + tl.seq * a.c.table_ld;
+  const int n_mine = max(0, hi - lo - warp + W - 1) / W, steps = (n_mine + P - 1) / P;
+  uint8_t* ring = kv4_smem + warp * (SLOTS * P * PB);
+  const uint64_t pol = l2_policy_evict_first();
+  // lane p < P: block of page p of a step (loaded one step before its copies go out)
+  auto load_id = [&](int step) {
+    const int k = step * P + lane;
+    return lane < P && k < n_mine ? __ldg(table + lo + warp + W * k) : -1;
+  };
+  int fill = 0;  // the slot that the next step's copies fill
+  auto issue = [&](int step, int id) {
+    if (step >= steps) return;
+    const int slot = fill, n = min(P, n_mine - step * P);
+    const bool good = id >= 0 && id < a.c.num_blocks;
+    const uint32_t in = __ballot_sync(0xffffffffu, lane < n && good);
+    uint8_t* dst = ring + slot * P * PB;
+    if (__popc(in) != n) {  // a page that the table does not name counts as zeros
+      for (int p = 0; p < n; ++p)
+        if (!((in >> p) & 1u))
+          for (int i = lane * 16; i < PB; i += 512) *reinterpret_cast<uint4*>(dst + p * PB + i) = make_uint4(0, 0, 0, 0);
+      if (lane == 0) kv4_error(a.c.status, kKv4BadTable);
+      fence_proxy_async_smem();  // before the slot's next copies
+    }
+    if (lane == 0) mbar_arrive_expect_tx(&bar[slot], static_cast<uint32_t>(__popc(in)) * PB);
+    __syncwarp();
+    if ((in >> lane) & 1u)
+      bulk_g2s(dst + lane * PB, a.c.pool + (static_cast<int64_t>(id) * a.c.n_kv + tl.g) * PB, PB, &bar[slot], pol);
+    fill = fill + 1 == SLOTS ? 0 : fill + 1;
+  };
+  bool waited = true;
+  uint32_t phase = 0;  // bit i: the parity that slot i completes next
+  auto wait = [&](int slot) {  // bounded; a wait that runs out sets the status
+    uint64_t* b = &bar[slot];
+    const uint32_t parity = (phase >> slot) & 1u;
+    phase ^= 1u << slot;
+    if (mbar_test(b, parity)) return;
+    const uint64_t t0 = globaltimer_ns();
+    for (uint32_t i = 1; !mbar_test(b, parity); ++i)
+      if ((i & 255u) == 0 && globaltimer_ns() - t0 > kKv4WaitNs) {
+        waited = false;
+        return;
+      }
+  };
+  int id = load_id(0);
+#pragma unroll
+  for (int st = 0; st < kKv4Ahead; ++st) {
+    const int next = load_id(st + 1);
+    issue(st, id);
+    id = next;
+  }
 
   // query fragments: column gid of each block, dims 64h + 16 tig .. in the codes' order
   uint32_t qf[NB][NH][8];
+  float up[NB][2];  // softmax scales of columns 2 tig, 2 tig + 1
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const int col = c0 + 8 * nb + gid;
     const bool in = col < cols;
-    const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(tl.r0 + (in ? col / tl.group : 0)) * a.q_row +
-                 static_cast<int64_t>(tl.g * tl.group + (in ? col % tl.group : 0)) * a.q_head + 16 * tig;
-    const bool vec = aligned16(a.q, a.q_row, a.q_head, sizeof(T));
-#pragma unroll
-    for (int h = 0; h < NH; ++h) {
-      __align__(16) T x[16];
-      if (!in) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = from_f32<T>(0.f);
-      } else if (vec) {
-        reinterpret_cast<uint4*>(x)[0] = *reinterpret_cast<const uint4*>(q + 64 * h);
-        reinterpret_cast<uint4*>(x)[1] = *reinterpret_cast<const uint4*>(q + 64 * h + 8);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = q[64 * h + i];
-      }
-      const uint16_t* b = reinterpret_cast<const uint16_t*>(x);
-#pragma unroll
-      for (int s = 0; s < 4; ++s) {  // k-step s: dims (s, s + 4) and (8 + s, 12 + s) of the 16
-        qf[nb][h][2 * s] = b[s] | (static_cast<uint32_t>(b[s + 4]) << 16);
-        qf[nb][h][2 * s + 1] = b[8 + s] | (static_cast<uint32_t>(b[12 + s]) << 16);
-      }
-    }
+    const int row = in && tl.rows > 1 ? kv4_row(a, col) : 0, head = in ? col - row * a.group : 0;
+    const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(tl.r0 + row) * a.q_row +
+                 static_cast<int64_t>(tl.g * a.group + head) * a.q_head + 16 * tig;
+    const float scale = a.scale_log2 * kv4_query<NH>(q, in, aligned16(a.q, a.q_row, a.q_head, sizeof(T)), qf[nb]);
+    up[nb][0] = __shfl_sync(0xffffffffu, scale, 8 * tig);
+    up[nb][1] = __shfl_sync(0xffffffffu, scale, 8 * tig + 4);
   }
   // columns 2 tig, 2 tig + 1 of each block: the positions they see
   int lim[NB][2];
@@ -525,115 +645,216 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const int col = c0 + 8 * nb + 2 * tig + e;
-      lim[nb][e] = col < cols ? tl.limit(col) : 0;
-      m[nb][e] = -INFINITY;
+      lim[nb][e] = col < cols ? kv4_limit(a, tl, col) : 0;
+      m[nb][e] = -INFINITY;  // of the scores before their scale
       l[nb][e] = 0.f;
     }
-  const int seen = tl.limit(min(cols, c0 + COLS) - 1);  // positions that any column sees
+  const int seen = kv4_limit(a, tl, min(cols, c0 + COLS) - 1);  // positions that any column sees
   float o[NB][4 * NH][4];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int j = 0; j < 4 * NH; ++j) o[nb][j][0] = o[nb][j][1] = o[nb][j][2] = o[nb][j][3] = 0.f;
 
-  const int32_t* table = a.c.table + tl.seq * a.c.table_ld;
-  for (int pg = lo + warp; pg < hi; pg += kKv4Warps) {
-    const int blk = __ldg(table + pg);
-    if (blk < 0 || blk >= a.c.num_blocks) {
-      if (lane == 0) kv4_error(a.c.status, kKv4BadTable);
-      continue;
-    }
-    const uint8_t* page = a.c.pool + (static_cast<int64_t>(blk) * a.c.n_kv + tl.g) * kv4_page_bytes(D);
-    float sc[NB][4];
+  const int all_see = kv4_limit(a, tl, c0);  // positions that every column sees
+  int slot = 0;
+  for (int step = 0; step < steps; ++step, slot = slot + 1 == SLOTS ? 0 : slot + 1) {
+    const int next = load_id(step + kKv4Ahead + 1);
+    issue(step + kKv4Ahead, id);
+    id = next;
+    wait(slot);
+    __syncwarp();
+    const uint8_t* page0 = ring + slot * P * PB;
+    const int n = min(P, n_mine - step * P);
+    const int at0 = (lo + warp + W * step * P) * kKv4Page;  // page p of the step starts at at0 + 16 W p
+    // No branch around the pages a last step lacks: their scores are masked and
+    // their V scales dropped below, whatever the ring holds.
+    float sc[P][NB][4];
 #pragma unroll
-    for (int nb = 0; nb < NB; ++nb) sc[nb][0] = sc[nb][1] = sc[nb][2] = sc[nb][3] = 0.f;
+    for (int p = 0; p < P; ++p) {
+      const uint8_t* page = page0 + p * PB;
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {
-      const uint4 kc = __ldg(reinterpret_cast<const uint4*>(page) + h * 32 + lane);
-      const uint32_t kb = __ldg(reinterpret_cast<const uint16_t*>(page + 8 * D) + h * 32 + lane);
-      const uint32_t s0 = Op::scale(__byte_perm(kb, 0u, 0x0404)), s1 = Op::scale(__byte_perm(kb, 0u, 0x1414));
-      const uint32_t f0 = Op::offset(s0), f1 = Op::offset(s1);
+      for (int h = 0; h < NH; ++h) {
+        const uint4 kc = reinterpret_cast<const uint4*>(page)[h * 32 + lane];
+        const uint32_t kb = reinterpret_cast<const uint16_t*>(page + 8 * D)[h * 32 + lane];
+        const uint32_t s0 = kv4_scales(kb, 0x4040), s1 = kv4_scales(kb, 0x4141);
+        uint32_t k0[4], k1[4], k2[4], k3[4];
+        kv4_values(kc.x, s0, k0);
+        kv4_values(kc.z, s1, k1);
+        kv4_values(kc.y, s0, k2);
+        kv4_values(kc.w, s1, k3);
 #pragma unroll
-      for (int s = 0; s < 4; ++s) {
-        const uint32_t k[4] = {Op::value(kc.x >> (4 * s), s0, f0), Op::value(kc.z >> (4 * s), s1, f1),
-                               Op::value(kc.y >> (4 * s), s0, f0), Op::value(kc.w >> (4 * s), s1, f1)};
+        for (int s = 0; s < 4; ++s)
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) Op::mma(sc[nb], k, qf[nb][h][2 * s], qf[nb][h][2 * s + 1]);
+          for (int nb = 0; nb < NB; ++nb) {
+            if (h == 0 && s == 0) mma_half_first(sc[p][nb], k0[s], k1[s], k2[s], k3[s], qf[nb][h][0], qf[nb][h][1]);
+            else mma_half(sc[p][nb], k0[s], k1[s], k2[s], k3[s], qf[nb][h][2 * s], qf[nb][h][2 * s + 1]);
+          }
       }
     }
-    // softmax of the page's 16 positions: rows gid (c0, c1) and gid + 8 (c2, c3)
-    uint32_t pf[NB][2];
-    const int p0 = pg * kKv4Page + gid;
+    // softmax of the step's positions: rows gid (c0, c1) and gid + 8 (c2, c3) of each page
+    const bool whole = n == P && at0 + W * kKv4Page * (P - 1) + kKv4Page <= all_see;
+    if (!whole) {
+#pragma unroll
+      for (int p = 0; p < P; ++p)
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int left = p < n ? lim[nb][e] - at0 - W * kKv4Page * p - gid : 0;  // > 0: row gid is seen
+            if (left <= 0) sc[p][nb][e] = -INFINITY;
+            if (left <= 8) sc[p][nb][2 + e] = -INFINITY;
+          }
+    }
+    uint32_t pf[P][NB][2];
 #pragma unroll
     for (int nb = 0; nb < NB; ++nb) {
-      float x[4], al[2];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) x[i] = p0 + 8 * (i >> 1) < lim[nb][i & 1] ? sc[nb][i] * a.scale_log2 : -INFINITY;
+      float al[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        float mx = fmaxf(x[e], x[2 + e]);
+        float mx = fmaxf(sc[0][nb][e], sc[0][nb][2 + e]);
+#pragma unroll
+        for (int p = 1; p < P; ++p) mx = fmaxf(mx, fmaxf(sc[p][nb][e], sc[p][nb][2 + e]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
         const float mn = fmaxf(m[nb][e], mx), ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: all zero
-        al[e] = exp2_fast(m[nb][e] - ref);
+        al[e] = exp2_fast((m[nb][e] - ref) * up[nb][e]);
         m[nb][e] = mn;
-        x[e] = exp2_fast(x[e] - ref + Op::kPOffset);
-        x[2 + e] = exp2_fast(x[2 + e] - ref + Op::kPOffset);
-        l[nb][e] = fmaf(l[nb][e], al[e], x[e] + x[2 + e]);
-      }
-      pf[nb][0] = transpose8x8(Op::pack(x[0], x[1]));
-      pf[nb][1] = transpose8x8(Op::pack(x[2], x[3]));
+        const float sub = fmaf(-ref, up[nb][e], kKv4POffset);
+        float sum = 0.f;
 #pragma unroll
-      for (int j = 0; j < 4 * NH; ++j) {
-        o[nb][j][0] *= al[0];
-        o[nb][j][1] *= al[1];
-        o[nb][j][2] *= al[0];
-        o[nb][j][3] *= al[1];
+        for (int p = 0; p < P; ++p) {
+          sc[p][nb][e] = exp2_fast(fmaf(sc[p][nb][e], up[nb][e], sub));
+          sc[p][nb][2 + e] = exp2_fast(fmaf(sc[p][nb][2 + e], up[nb][e], sub));
+          sum += sc[p][nb][e] + sc[p][nb][2 + e];
+        }
+        l[nb][e] = fmaf(l[nb][e], al[e], sum);
+      }
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        pf[p][nb][0] = transpose8x8(pack_half2(sc[p][nb][0], sc[p][nb][1]));
+        pf[p][nb][1] = transpose8x8(pack_half2(sc[p][nb][2], sc[p][nb][3]));
+      }
+      if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {  // a maximum grew
+#pragma unroll
+        for (int j = 0; j < 4 * NH; ++j) {
+          o[nb][j][0] *= al[0];
+          o[nb][j][1] *= al[1];
+          o[nb][j][2] *= al[0];
+          o[nb][j][3] *= al[1];
+        }
       }
     }
     // positions past the last one seen may never have been written: their V
     // scales are dropped, since 0 times an infinity or a NaN is not 0
-    uint32_t keep = 0xFFFFFFFFu;
-    const int left = seen - pg * kKv4Page;
-    if (left < kKv4Page) {
-      keep = 0u;
+    uint32_t keep[P];
 #pragma unroll
-      for (int i = 0; i < 4; ++i)
-        if (2 * tig + 8 * (i >> 1) + (i & 1) < left) keep |= 0xFFu << (8 * i);
-    }
+    for (int p = 0; p < P; ++p) keep[p] = 0xFFFFFFFFu;
+    if (!whole) {
 #pragma unroll
-    for (int h = 0; h < NH; ++h) {
-      const uint4 vc = __ldg(reinterpret_cast<const uint4*>(page + 9 * D) + h * 32 + lane);
-      const uint32_t vb =
-          __ldg(reinterpret_cast<const uint32_t*>(page + 17 * D) + (h * 4 + (gid >> 1)) * 4 + tig) & keep;
-      const uint32_t s0 = Op::scale(__byte_perm(vb, 0u, 0x1404)), s1 = Op::scale(__byte_perm(vb, 0u, 0x3424));
-      const uint32_t f0 = Op::offset(s0), f1 = Op::offset(s1);
+      for (int p = 0; p < P; ++p) {
+        const int left = p < n ? seen - at0 - W * kKv4Page * p : 0;
+        keep[p] = 0u;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {  // dims 2j (row gid) and 2j + 1 (row gid + 8) of the lane's 8
-        const uint32_t w0 = j < 2 ? vc.x : vc.y, w1 = j < 2 ? vc.z : vc.w;
-        const int sh = 8 * (j & 1);
-        const uint32_t v[4] = {Op::value(w0 >> sh, s0, f0), Op::value(w0 >> (sh + 4), s0, f0),
-                               Op::value(w1 >> sh, s1, f1), Op::value(w1 >> (sh + 4), s1, f1)};
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) Op::mma(o[nb][4 * h + j], v, pf[nb][0], pf[nb][1]);
+        for (int i = 0; i < 4; ++i)
+          if (2 * tig + 8 * (i >> 1) + (i & 1) < left) keep[p] |= 0xFFu << (8 * i);
       }
     }
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+      const uint8_t* page = page0 + p * PB;
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        const uint4 vc = reinterpret_cast<const uint4*>(page + 9 * D)[h * 32 + lane];
+        const uint32_t vb = reinterpret_cast<const uint32_t*>(page + 17 * D)[(h * 4 + (gid >> 1)) * 4 + tig] & keep[p];
+        const uint32_t s0 = kv4_scales(vb, 0x4140), s1 = kv4_scales(vb, 0x4342);
+        // word (positions 2 tig, + 1 or 2 tig + 8, + 9; dims 0-3 or 4-7 of the lane's 8)
+        uint32_t v0[4], v1[4], w0[4], w1[4];
+        kv4_values(vc.x, s0, v0);
+        kv4_values(vc.z, s1, w0);
+        kv4_values(vc.y, s0, v1);
+        kv4_values(vc.w, s1, w1);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {  // block j: dims 2j (row gid) and 2j + 1 (row gid + 8)
+          mma_half(o[nb][4 * h], v0[0], v0[1], w0[0], w0[1], pf[p][nb][0], pf[p][nb][1]);
+          mma_half(o[nb][4 * h + 1], v0[2], v0[3], w0[2], w0[3], pf[p][nb][0], pf[p][nb][1]);
+          mma_half(o[nb][4 * h + 2], v1[0], v1[1], w1[0], w1[1], pf[p][nb][0], pf[p][nb][1]);
+          mma_half(o[nb][4 * h + 3], v1[2], v1[3], w1[2], w1[3], pf[p][nb][0], pf[p][nb][1]);
+        }
+      }
+    }
+    __syncwarp();  // every lane is done with the step's pages before they are refilled
   }
-
-  // the warps' states to shared memory: column 2 tig + e, dims 64h + 8 gid ..
+  if (!__all_sync(0xffffffffu, waited)) {
+    // a wait ran out: the result means nothing; wait once more for what is in flight
+    if (lane == 0) kv4_error(a.c.status, kKv4Timeout);
+    for (int i = 0; i < SLOTS; ++i)
+      if (i < steps) {
+        phase ^= 1u << i;  // the slot's last phase once more
+        wait(i);
+      }
+  }
+  // ---- the result: column 2 tig + e of each block, dims 64h + 8 gid .. in this lane ----
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      float s = l[nb][e];
-      s += __shfl_xor_sync(0xffffffffu, s, 4);
-      s += __shfl_xor_sync(0xffffffffu, s, 8);
-      s += __shfl_xor_sync(0xffffffffu, s, 16);
+      l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 4);
+      l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 8);
+      l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 16);
+    }
+  const bool ovec = aligned16(a.out, a.o_row, a.o_head, sizeof(T));
+  // 8 dims from d0 of column c (of the sequence): final, or this split's share
+  auto put = [&](int c, int d0, float (&r)[8], float M, float L) {
+    if (a.splits == 1) {
+      const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);  // a row that sees nothing: zeros (NaN stays NaN)
+#pragma unroll
+      for (int k = 0; k < 8; ++k) r[k] *= inv;
+      const int row = tl.rows > 1 ? kv4_row(a, c) : 0;
+      store8(static_cast<T*>(a.out) + static_cast<int64_t>(tl.r0 + row) * a.o_row +
+                 static_cast<int64_t>(tl.g * a.group + c - row * a.group) * a.o_head + d0,
+             r, ovec);
+    } else {
+      float* dst = kv4_part(a, tl.seq, tl.g, tl.tile, tl.split, c - c0, D);
+      *reinterpret_cast<float4*>(dst + d0) = make_float4(r[0], r[1], r[2], r[3]);
+      *reinterpret_cast<float4*>(dst + d0 + 4) = make_float4(r[4], r[5], r[6], r[7]);
+      if (d0 == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(M, L);
+    }
+  };
+  if constexpr (W == 1) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int c = c0 + 8 * nb + 2 * tig + e;
+        if (c >= cols) continue;
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          float r[8];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            r[2 * j] = o[nb][4 * h + j][e];
+            r[2 * j + 1] = o[nb][4 * h + j][2 + e];
+          }
+          put(c, 64 * h + 8 * gid, r, m[nb][e] * up[nb][e], l[nb][e]);
+        }
+      }
+    return;
+  }
+  __syncthreads();  // the ring's memory becomes the warps' states
+  float(*s_o)[COLS][D] = reinterpret_cast<float(*)[COLS][D]>(kv4_smem);
+  float(*s_m)[COLS] = reinterpret_cast<float(*)[COLS]>(kv4_smem + sizeof(float) * W * COLS * D);
+  float(*s_l)[COLS] = s_m + W;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
       const int col = 8 * nb + 2 * tig + e;
+      if (c0 + col >= cols) continue;
       if (gid == 0) {
-        s_m[warp][col] = m[nb][e];
-        s_l[warp][col] = s;
+        s_m[warp][col] = m[nb][e] * up[nb][e];
+        s_l[warp][col] = l[nb][e];
       }
 #pragma unroll
       for (int h = 0; h < NH; ++h) {
@@ -643,61 +864,43 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
       }
     }
   __syncthreads();
-  const int64_t unit = (static_cast<int64_t>(tl.seq) * a.c.n_kv + tl.g) * a.tiles + tl.tile;
-  const bool ovec = aligned16(a.out, a.o_row, a.o_head, sizeof(T));
-  for (int i = threadIdx.x; i < COLS * (D / 8); i += 32 * kKv4Warps) {
+  for (int i = threadIdx.x; i < COLS * (D / 8); i += 32 * W) {
     const int col = i / (D / 8), d0 = i % (D / 8) * 8;
     if (c0 + col >= cols) break;
     float M = s_m[0][col], L = 0.f, r[8];
 #pragma unroll
-    for (int w = 1; w < kKv4Warps; ++w) M = fmaxf(M, s_m[w][col]);
+    for (int w = 1; w < W; ++w) M = fmaxf(M, s_m[w][col]);
 #pragma unroll
     for (int k = 0; k < 8; ++k) r[k] = 0.f;
     const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
-    for (int w = 0; w < kKv4Warps; ++w) {
+    for (int w = 0; w < W; ++w) {
       const float f = exp2_fast(s_m[w][col] - ref);
       L = fmaf(f, s_l[w][col], L);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) r[k] = fmaf(f, s_o[w][col][d0 + k], r[k]);
+      const float4 x = *reinterpret_cast<const float4*>(&s_o[w][col][d0]), y = *reinterpret_cast<const float4*>(&s_o[w][col][d0 + 4]);
+      r[0] = fmaf(f, x.x, r[0]); r[1] = fmaf(f, x.y, r[1]); r[2] = fmaf(f, x.z, r[2]); r[3] = fmaf(f, x.w, r[3]);
+      r[4] = fmaf(f, y.x, r[4]); r[5] = fmaf(f, y.y, r[5]); r[6] = fmaf(f, y.z, r[6]); r[7] = fmaf(f, y.w, r[7]);
     }
-    if (a.splits == 1) {
-      const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);  // a row that sees nothing: zeros (NaN stays NaN)
-#pragma unroll
-      for (int k = 0; k < 8; ++k) r[k] *= inv;
-      const int c = c0 + col;
-      store8(static_cast<T*>(a.out) + static_cast<int64_t>(tl.r0 + c / tl.group) * a.o_row +
-                 static_cast<int64_t>(tl.g * tl.group + c % tl.group) * a.o_head + d0,
-             r, ovec);
-    } else {
-      float* dst = a.part + ((unit * a.splits + tl.split) * COLS + col) * (D + 4);
-      *reinterpret_cast<float4*>(dst + d0) = make_float4(r[0], r[1], r[2], r[3]);
-      *reinterpret_cast<float4*>(dst + d0 + 4) = make_float4(r[4], r[5], r[6], r[7]);
-      if (d0 == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(M, L);
-    }
+    put(c0 + col, d0, r, M, L);
   }
 }
 
-// Joins the splits of each column, in split order: one warp per column.
-template <class Op, int NH, int NB>
-__global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
-  using T = typename Op::T;
-  constexpr int D = 64 * NH, COLS = 8 * NB, PER = D / 32;
+// Joins the splits of each column: one CTA per column, its warps take the
+// splits w, w + 4, .. (8 loads in flight a lane), then meet in warp order.
+template <class T, int NH>
+__global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
+  constexpr int D = 64 * NH, PER = 2 * NH, WARPS = 4, DEEP = 8;
+  __shared__ float s_r[WARPS][D], s_l[WARPS];
   pdl_wait();
   pdl_launch();
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-  const int lane = threadIdx.x & 31, col = static_cast<int>(i % COLS);
-  const int64_t unit = i / COLS;
-  if (unit >= static_cast<int64_t>(a.n_seqs) * a.c.n_kv * a.tiles) return;
+  // grid: x = sequence, y = kv head, z = column
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int c = blockIdx.z, tile = c / a.tile_cols;
   Kv4Tile tl;
-  // the unit's first split, in the numbering of the attention kernel's CTAs
-  const int tile = static_cast<int>(unit % a.tiles);
-  if (!kv4_tile(a, static_cast<int>((unit / a.tiles) * a.splits * a.tiles + tile), COLS, tl)) return;
-  const int c = tl.tile * COLS + col;
-  if (c >= tl.cols()) return;
-  const int n = max(1, (kv4_tile_pages(tl, COLS) + a.split_pages - 1) / a.split_pages);
-  const float* src = a.part + (unit * a.splits * COLS + col) * (D + 4);
-  const int64_t step = static_cast<int64_t>(COLS) * (D + 4);
+  if (!kv4_tile(a, tile, tl) || c >= tl.cols(a)) return;
+  const int n = max(1, (kv4_tile_pages(a, tl) + a.split_pages - 1) / a.split_pages);
+  const float* src = kv4_part(a, tl.seq, tl.g, tile, 0, c - tile * a.tile_cols, D);
+  const int64_t step = static_cast<int64_t>(a.tile_cols) * (D + 4);
   float M = -INFINITY;
   for (int s = lane; s < n; s += 32) M = fmaxf(M, src[s * step + D]);
 #pragma unroll
@@ -706,18 +909,40 @@ __global__ void __launch_bounds__(256) kv4_join_kernel(const __grid_constant__ K
   float L = 0.f, r[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) r[k] = 0.f;
-  for (int s = 0; s < n; ++s) {
-    const float2 ml = *reinterpret_cast<const float2*>(src + s * step + D);
-    const float f = exp2_fast(ml.x - ref);
-    L = fmaf(f, ml.y, L);
+  for (int s0 = warp; s0 < n; s0 += WARPS * DEEP) {
+    float2 ml[DEEP], x[DEEP][NH];
 #pragma unroll
-    for (int k = 0; k < PER; ++k) r[k] = fmaf(f, src[s * step + lane + 32 * k], r[k]);
+    for (int i = 0; i < DEEP; ++i) {
+      const int s = s0 + WARPS * i;
+      ml[i] = s < n ? *reinterpret_cast<const float2*>(src + s * step + D) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+        x[i][h] = s < n ? *reinterpret_cast<const float2*>(src + s * step + 64 * h + 2 * lane) : make_float2(0.f, 0.f);
+    }
+#pragma unroll
+    for (int i = 0; i < DEEP; ++i) {
+      const float f = exp2_fast(ml[i].x - ref);
+      L = fmaf(f, ml[i].y, L);
+#pragma unroll
+      for (int h = 0; h < NH; ++h) {
+        r[2 * h] = fmaf(f, x[i][h].x, r[2 * h]);
+        r[2 * h + 1] = fmaf(f, x[i][h].y, r[2 * h + 1]);
+      }
+    }
   }
-  const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
-  T* out = static_cast<T*>(a.out) + static_cast<int64_t>(tl.r0 + c / tl.group) * a.o_row +
-           static_cast<int64_t>(tl.g * tl.group + c % tl.group) * a.o_head;
 #pragma unroll
-  for (int k = 0; k < PER; ++k) out[lane + 32 * k] = from_f32<T>(r[k] * inv);
+  for (int h = 0; h < NH; ++h) *reinterpret_cast<float2*>(&s_r[warp][64 * h + 2 * lane]) = make_float2(r[2 * h], r[2 * h + 1]);
+  if (lane == 0) s_l[warp] = L;
+  __syncthreads();
+  if (threadIdx.x < D) {
+    const int d = threadIdx.x;
+    L = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
+    const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
+    const int row = kv4_row(a, c);
+    static_cast<T*>(a.out)[static_cast<int64_t>(tl.r0 + row) * a.o_row +
+                           static_cast<int64_t>(tl.g * a.group + c - row * a.group) * a.o_head + d] =
+        from_f32<T>(((s_r[0][d] + s_r[1][d]) + (s_r[2][d] + s_r[3][d])) * inv);
+  }
 }
 
 }  // namespace b2d

@@ -58,12 +58,16 @@ struct Kv4AttnArgs {
   // set by kv4_attn_plan: query columns (row, head) per tile, tiles per
   // (sequence, kv head), splits of the positions and pages per split
   int tile_cols, tiles, splits, split_pages;
+  int warps;               // of a CTA (1, 2 or 4)
+  int group;               // query heads of a kv head
+  uint64_t group_inv;      // ceil(2^32 / group): c / group = c * group_inv >> 32 while c * group < 2^32
 };
 
 cudaError_t kv4_append(const Kv4AppendArgs& a, cudaStream_t st, bool pdl);
 cudaError_t kv4_read(const Kv4ReadArgs& a, cudaStream_t st);
-// The split of a call's work, then the bytes of a.part it needs.
-void kv4_attn_plan(Kv4AttnArgs& a, int sms);
+// The split of a call's work (false: too large for a grid), then the bytes of
+// a.part it needs.
+bool kv4_attn_plan(Kv4AttnArgs& a, int sms);
 uint64_t kv4_attn_scratch(const Kv4AttnArgs& a);
 cudaError_t kv4_attention(const Kv4AttnArgs& a, cudaStream_t st, bool pdl);
 
