@@ -3,8 +3,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
-#include <cstdlib>
-#include <cstdlib>
 #include <cstring>
 
 #include "b2d_host.h"
@@ -16,12 +14,18 @@ namespace {
 
 template <class T, class TQ>
 cudaError_t append_typed(const Kv4AppendArgs& a, cudaStream_t st, bool pdl) {
-  const int slices = kKv4AppendThreads / (a.c.d / kKv4Group);
-  const int total = (a.q ? a.n_heads : 0) + 2 * a.c.n_kv;
-  // one head a thread until the rows alone fill the GPU's threads several times over
-  const int heads = a.n_rows >= 2048 ? total : slices;
-  const dim3 grid(static_cast<unsigned>(a.n_rows), static_cast<unsigned>((total + heads - 1) / heads));
-  return launch(kv4_append_kernel<T, TQ>, grid, dim3(kKv4AppendThreads), 0, st, pdl, a, heads);
+  // Many rows: a warp takes a whole row, so its addresses and angles are worked
+  // out once (10242 rows: 98 us with the read-back, 108 with four warps a row);
+  // few: a block per batch of heads, one head a thread (512 rows: 7.7 us).
+  const bool many = a.n_rows >= 2048;
+  const int threads = many ? 32 : kKv4AppendThreads;
+  const int slices = threads / (a.c.d / 8);
+  const unsigned batches = many ? 1u : static_cast<unsigned>((a.n_heads + slices - 1) / slices + 2);
+  const dim3 grid(static_cast<unsigned>(a.n_rows), batches), block(threads);
+  if (!a.cos) return launch(kv4_append_kernel<T, TQ, kRopeNone>, grid, block, 0, st, pdl, a);
+  if (a.interleaved) return launch(kv4_append_kernel<T, TQ, kRopePairs>, grid, block, 0, st, pdl, a);
+  if (a.rotary % 16 == 0) return launch(kv4_append_kernel<T, TQ, kRopeBlocks>, grid, block, 0, st, pdl, a);
+  return launch(kv4_append_kernel<T, TQ, kRopeAny>, grid, block, 0, st, pdl, a);
 }
 
 // Dynamic shared memory past 48 KB is granted per kernel and device, once.
@@ -38,13 +42,13 @@ cudaError_t raise_smem() {
   return e;
 }
 
-template <class T, int NH, int NB, int W>
+template <class T, int NH, int NB>
 cudaError_t attn_launch(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
-  constexpr int smem = kv4_attn_smem<NH, NB, W>();
-  cudaError_t e = raise_smem<kv4_attn_kernel<T, NH, NB, W>, smem>();
+  constexpr int smem = kv4_attn_smem<NH, NB>();
+  cudaError_t e = raise_smem<kv4_attn_kernel<T, NH, NB>, smem>();
   const unsigned x = static_cast<unsigned>(a.n_seqs), y = static_cast<unsigned>(a.c.n_kv);
   if (e == cudaSuccess)
-    e = launch(kv4_attn_kernel<T, NH, NB, W>, dim3(x, y, static_cast<unsigned>(a.tiles * a.splits)), dim3(32 * W), smem,
+    e = launch(kv4_attn_kernel<T, NH, NB>, dim3(x, y, static_cast<unsigned>(a.tiles * a.splits)), dim3(32 * kKv4Warps), smem,
                st, pdl, a);
   if (e == cudaSuccess && a.splits > 1)
     e = launch(kv4_join_kernel<T, NH>, dim3(x, y, static_cast<unsigned>(a.max_rows * a.group)), dim3(128), 0, st, true,
@@ -54,10 +58,7 @@ cudaError_t attn_launch(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
 
 template <class T, int NH>
 cudaError_t attn_shape(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
-  if (a.tile_cols > 8) return attn_launch<T, NH, 2, 4>(a, st, pdl);
-  if (a.warps == 1) return attn_launch<T, NH, 1, 1>(a, st, pdl);
-  if (a.warps == 2) return attn_launch<T, NH, 1, 2>(a, st, pdl);
-  return attn_launch<T, NH, 1, 4>(a, st, pdl);
+  return a.tile_cols > 8 ? attn_launch<T, NH, 2>(a, st, pdl) : attn_launch<T, NH, 1>(a, st, pdl);
 }
 
 template <class T>
@@ -79,9 +80,11 @@ cudaError_t kv4_append(const Kv4AppendArgs& a, cudaStream_t st, bool pdl) {
 }
 
 cudaError_t kv4_read(const Kv4ReadArgs& a, cudaStream_t st) {
-  const int64_t n = static_cast<int64_t>(a.n_rows) * a.c.n_kv * 2 * (a.c.d / kKv4Group);
-  if (n == 0) return cudaSuccess;
-  const dim3 grid(static_cast<unsigned>((n + 255) / 256)), block(256);
+  if (a.n_rows == 0) return cudaSuccess;
+  const int slices = 128 / (a.c.d / 8);
+  const dim3 grid(static_cast<unsigned>(a.n_rows),
+                  a.n_rows >= 2048 ? 1u : static_cast<unsigned>(std::min(65535, (2 * a.c.n_kv + slices - 1) / slices))),
+      block(128);
   if (a.dtype == B2D_F32) return launch(kv4_read_kernel<float>, grid, block, 0, st, false, a);
   if (a.dtype == B2D_F16) return launch(kv4_read_kernel<__half>, grid, block, 0, st, false, a);
   return launch(kv4_read_kernel<__nv_bfloat16>, grid, block, 0, st, false, a);
@@ -104,8 +107,6 @@ bool kv4_attn_plan(Kv4AttnArgs& a, int sms) {
   const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(ctas / std::max<int64_t>(1, units), (pages + 31) / 32));
   a.split_pages = static_cast<int>((pages + splits - 1) / splits);
   a.splits = (pages + a.split_pages - 1) / a.split_pages;
-  a.warps = 4;
-  if (getenv("KV4_W")) a.warps = atoi(getenv("KV4_W"));
   // the grid's y and z
   return a.c.n_kv <= 65535 && int64_t(a.tiles) * a.splits <= 65535 && (a.splits == 1 || cols <= 65535);
 }
@@ -129,8 +130,6 @@ namespace {
     cudaError_t e_ = (call);                              \
     if (e_ != cudaSuccess) return b2d::cuda_failed(e_, what); \
   } while (0)
-
-constexpr int64_t kMaxBlocks = 0x7fffffff;  // CTAs of a launch
 
 b2d_status check_cache(const b2d_kv4_cache* c, b2d::Kv4Cache& k) {
   if (!c || !c->pool || (reinterpret_cast<uintptr_t>(c->pool) & 15u) || !c->table || c->n_kv_heads < 1 ||
@@ -222,7 +221,6 @@ extern "C" b2d_status b2d_kv4_read(const b2d_kv4_cache* cache, const int32_t* po
   if (s != B2D_OK) return s;
   if (!pos_dev || !k_dev || !v_dev || n_rows < 0 || (!seq_dev && n_rows > cache->table_rows)) return B2D_ERR_INVALID_ARG;
   if (dtype < B2D_F32 || dtype > B2D_F16) return B2D_ERR_UNSUPPORTED;
-  if (int64_t(n_rows) * a.c.n_kv * 2 * (a.c.d / b2d::kKv4Group) > kMaxBlocks * 256) return B2D_ERR_UNSUPPORTED;
   a.k = k_dev; a.v = v_dev; a.pos = pos_dev; a.seq = seq_dev;
   a.n_rows = n_rows;
   a.dtype = dtype;

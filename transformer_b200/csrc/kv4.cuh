@@ -87,18 +87,21 @@ __device__ __forceinline__ __half from_f32(float x) { return __float2half_rn(x);
 
 // 8 elements from / to p; vec: p is 16-byte aligned.
 template <class T>
-__device__ __forceinline__ void load8(const T* p, float* x, bool vec) {
+struct __align__(16) Eight {
+  T v[8];
+};
+template <class T>
+__device__ __forceinline__ Eight<T> load8(const T* p, bool vec) {
+  Eight<T> x;
   if (vec) {
-    __align__(16) T v[8];
 #pragma unroll
     for (int i = 0; i < static_cast<int>(sizeof(T)) / 2; ++i)
-      reinterpret_cast<uint4*>(v)[i] = __ldg(reinterpret_cast<const uint4*>(p) + i);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(v[i]);
+      reinterpret_cast<uint4*>(x.v)[i] = reinterpret_cast<const uint4*>(p)[i];  // (not the read-only path: q may be q_out)
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = to_f32(p[i]);
+    for (int i = 0; i < 8; ++i) x.v[i] = p[i];
   }
+  return x;
 }
 template <class T>
 __device__ __forceinline__ void store8(T* p, const float* x, bool vec) {
@@ -112,6 +115,27 @@ __device__ __forceinline__ void store8(T* p, const float* x, bool vec) {
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) p[i] = from_f32<T>(x[i]);
+  }
+}
+// 8 values as four pairs of halves to p (all types hold them exactly).
+template <class T>
+__device__ __forceinline__ void put8(T* p, const uint32_t (&h)[4], bool vec) {
+  float x[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h[i]));
+    x[2 * i] = f.x;
+    x[2 * i + 1] = f.y;
+  }
+  store8(p, x, vec);
+}
+template <>
+__device__ __forceinline__ void put8(__half* p, const uint32_t (&h)[4], bool vec) {
+  if (vec) {
+    *reinterpret_cast<uint4*>(p) = make_uint4(h[0], h[1], h[2], h[3]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = __ushort_as_half(static_cast<unsigned short>(h[i >> 1] >> (16 * (i & 1))));
   }
 }
 __device__ __forceinline__ bool aligned16(const void* p, int64_t stride_a, int64_t stride_b, int size) {
@@ -136,27 +160,23 @@ __device__ __forceinline__ void rotate_pair(float x, float c, float y, float s, 
   }
 }
 
-// Scale byte of a group whose largest magnitude is m + ml (ml: the low part).
-// The quotient is rounded up, so rounding it up again to 4 bits gives the
-// smallest scale s with 7 s >= m exactly; where 7 s = m the low part decides.
-__device__ __forceinline__ uint32_t kv4_scale_byte(float m, float ml) {
-  const float q = __fdiv_ru(m, 7.f);
-  uint32_t b;
-  if (q >= 6.103515625e-05f) {  // 2^-14: normal
-    b = ((__float_as_uint(q) + 0xFFFFFu) >> 20) - (112u << 3);
-  } else {
-    b = static_cast<uint32_t>(ceilf(q * 131072.f));  // whole multiples of 2^-17 (exact product)
-  }
-  b = min(b, static_cast<uint32_t>(kKv4MaxByte));
-  if (ml > 0.f && 7.f * kv4_scale_value(b) == m && b < kKv4MaxByte) ++b;
+// Scale byte of a group whose largest magnitude is m: rounding up an estimate
+// just below m / 7 gives the byte or the one under it, and 7 s, exact in
+// float32, says which.  (A part below m's last bit can only matter where 7 s = m.)
+__device__ __forceinline__ uint32_t kv4_scale_byte(float m) {
+  const float q = m * 0.14285711f;  // (1 - 2^-22) / 7, rounded down
+  const uint32_t normal = ((__float_as_uint(q) + 0xFFFFFu) >> 20) - (112u << 3);
+  const uint32_t small = static_cast<uint32_t>(ceilf(q * 131072.f));  // below 2^-14: multiples of 2^-17
+  uint32_t b = min(q >= 6.103515625e-05f ? normal : small, static_cast<uint32_t>(kKv4MaxByte));
+  if (7.f * kv4_scale_value(b) < m && b < kKv4MaxByte) ++b;
   return b;
 }
 
-// Code (1..15) of hi + lo under scale s > 0 (inv = 1 / s).  The quotient may be
-// one off next to a half; the remainder hi - n s is exact (s has 4 bits, n few)
-// and settles it, ties by the low part, then to even.
-__device__ __forceinline__ uint32_t kv4_code(float hi, float lo, float s, float inv) {
-  float n = rintf(__fmul_rn(hi, inv));
+// Code (1..15) of hi + lo under scale s > 0, whatever they are: the quotient may
+// be one off next to a half; the remainder hi - n s is exact (s has 4 bits, n
+// few) and settles it, ties by the low part, then to even.
+__device__ __noinline__ uint32_t kv4_code_any(float hi, float lo, float s) {
+  float n = rintf(__fdiv_rn(hi, s));
   const float r = __fmaf_rn(-n, s, hi), half = 0.5f * s;
   const bool odd = (__float2int_rn(n) & 1) != 0;
   if (r > half || (r == half && (lo > 0.f || (lo == 0.f && odd)))) n += 1.f;
@@ -166,205 +186,66 @@ __device__ __forceinline__ uint32_t kv4_code(float hi, float lo, float s, float 
   return static_cast<uint32_t>(__float2int_rn(n) + 8);
 }
 
-// One group: 16 values as hi + lo -> scale byte and 16 nibbles (dim i in nibble i).
-__device__ __forceinline__ uint32_t kv4_quantise(const float (&hi)[16], const float (&lo)[16], uint2& codes) {
-  float m = 0.f, ml = 0.f;
+__device__ __forceinline__ float max_nan(float a, float b) {  // NaN if either is
+  float m;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(m) : "f"(a), "f"(b));
+  return m;
+}
+// Half a group: this lane's 8 values as hi + lo, the other half in lane ^ 1.
+// Returns the group's scale byte and the lane's 8 nibbles (dim i in nibble i).
+// few (the same for both lanes): lo is zero and hi has at most 11 significant bits.
+// The whole warp takes part.
+__device__ __forceinline__ uint32_t kv4_quantise(const float (&hi)[8], const float (&lo)[8], bool few,
+                                                 uint32_t& codes) {
+  float m = fabsf(hi[0]);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float a = fabsf(hi[i]), l = hi[i] < 0.f ? -lo[i] : lo[i];
-    if (a > m || (a == m && l > ml)) {
-      m = a;
-      ml = l;
+  for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(hi[i]));
+  m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  const uint32_t b = kv4_scale_byte(m);
+  const float s = kv4_scale_value(b);
+  // hi / s to the nearest whole number by adding 1.5 2^23 (and 8, the code's own
+  // offset), from an estimate a little above and one a little below: where they
+  // agree they are right.  Where not, the quotient is next to a half: with few
+  // bits it is on it (others are 2^-12 off), and the even number holds.
+  constexpr float kRound = 12582920.f;
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(s));
+  const float above = inv * (1.f + 0x1p-20f), below = inv * (1.f - 0x1p-20f);
+  uint32_t differ = 0u;
+  codes = 0u;
+#pragma unroll
+  for (int i = 7; i >= 0; --i) {
+    const uint32_t t = __float_as_uint(__fmaf_rn(hi[i], above, kRound));
+    const uint32_t u = __float_as_uint(__fmaf_rn(hi[i], below, kRound));
+    differ |= t ^ u;
+    codes = codes * 16u + ((t & 1u) ? u : t);
+  }
+  codes -= 0x4B400000u * 0x11111111u;  // each number's bits are 0x4B400000 + 8 + n
+  // zero and capped scales (a NaN has the capped byte), and what the low parts decide, are for below
+  const bool sure = b - 1u < kKv4MaxByte - 1u && (few || (differ == 0u && 7.f * s != m));
+  if (__all_sync(0xffffffffu, sure)) return b;
+  m = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = fmaxf(m, fabsf(hi[i]));  // (NaN counts for nothing)
+  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  uint32_t c = kv4_scale_byte(m);
+  float t = kv4_scale_value(c);
+  bool over = false;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) over = over || (hi[i] == m && lo[i] > 0.f) || (hi[i] == -m && lo[i] < 0.f);
+  const uint32_t votes = __ballot_sync(0xffffffffu, over) >> (threadIdx.x & 30);
+  if ((votes & 3u) && 7.f * t == m && c < kKv4MaxByte) t = kv4_scale_value(++c);
+  if (!sure) {
+    codes = c == 0u ? 0x88888888u : 0u;
+    if (c != 0u) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) codes |= kv4_code_any(hi[i], lo[i], t) << (4 * i);
     }
   }
-  const uint32_t b = kv4_scale_byte(m, ml);
-  codes = make_uint2(0x88888888u, 0x88888888u);
-  if (b != 0) {
-    const float s = kv4_scale_value(b), inv = __frcp_rn(s);
-    codes = make_uint2(0u, 0u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      codes.x |= kv4_code(hi[i], lo[i], s, inv) << (4 * i);
-      codes.y |= kv4_code(hi[8 + i], lo[8 + i], s, inv) << (4 * i);
-    }
-  }
-  return b;
+  return c;
 }
 
-// ---- append ------------------------------------------------------------------------
-// Thread = (group of 16 dims, slice of the heads): block of 128 threads, d / 16
-// groups x 2048 / d slices; blockIdx.x = row, blockIdx.y = batch of heads.
-// Heads are numbered q 0.., then k, then v; a thread keeps its 16 dims' angles
-// in registers over the heads it walks.
-constexpr int kKv4AppendThreads = 128;
-
-template <class T, class TQ>
-__global__ void __launch_bounds__(kKv4AppendThreads) kv4_append_kernel(const __grid_constant__ Kv4AppendArgs a,
-                                                                       int heads_per_block) {
-  pdl_wait();
-  pdl_launch();
-  const int groups = a.c.d >> 4;
-  const int grp = threadIdx.x % groups, slice = threadIdx.x / groups, slices = kKv4AppendThreads / groups;
-  const int row = blockIdx.x, i0 = grp * 16;
-  const int nq = a.q != nullptr ? a.n_heads : 0, total = nq + 2 * a.c.n_kv;
-  const int pos = a.pos[row];
-  if (pos < 0) return;  // idle row
-  const int sid = a.seq != nullptr ? a.seq[row] : row;
-  if (a.cos != nullptr && pos >= a.max_pos) {
-    if (threadIdx.x == 0) kv4_error(a.c.status, kKv4BadPos);
-    return;
-  }
-  const int half = a.rotary >> 1;
-  const bool rotate = a.cos != nullptr && i0 < a.rotary;
-  const bool blocks = (half & 7) == 0;  // a block of 8 dims has its partners in one block of 8
-  float c[16], s[16];  // out[i] = x[i] c[i] + partner[i] s[i]
-  if (rotate) {
-    const float* cr = a.cos + static_cast<int64_t>(pos) * half;
-    const float* sr = a.sin + static_cast<int64_t>(pos) * half;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) {
-      const int dim = i0 + i;
-      c[i] = 1.f;
-      s[i] = 0.f;
-      if (dim < a.rotary) {
-        const int f = a.interleaved ? dim >> 1 : dim < half ? dim : dim - half;
-        const bool first = a.interleaved ? (dim & 1) == 0 : dim < half;
-        c[i] = __ldg(cr + f);
-        s[i] = first ? -__ldg(sr + f) : __ldg(sr + f);
-      }
-    }
-  }
-  const bool qvec = aligned16(a.q, a.q_row, a.q_head, sizeof(T)), kvec = aligned16(a.k, a.k_row, a.k_head, sizeof(T));
-  const bool vvec = aligned16(a.v, a.v_row, a.v_head, sizeof(T));
-  const bool ovec = aligned16(a.q_out, a.qo_row, a.qo_head, sizeof(TQ));
-  const int lo_h = blockIdx.y * heads_per_block, hi_h = min(total, lo_h + heads_per_block);
-  for (int hh = lo_h + slice; hh < hi_h; hh += slices) {
-    const int kind = hh < nq ? 0 : hh < nq + a.c.n_kv ? 1 : 2;  // q, k, v
-    const int g = kind == 0 ? hh : kind == 1 ? hh - nq : hh - nq - a.c.n_kv;
-    const T* x = kind == 0   ? static_cast<const T*>(a.q) + row * a.q_row + g * a.q_head
-                 : kind == 1 ? static_cast<const T*>(a.k) + row * a.k_row + g * a.k_head
-                             : static_cast<const T*>(a.v) + row * a.v_row + g * a.v_head;
-    const bool vec = kind == 0 ? qvec : kind == 1 ? kvec : vvec;
-    float hi[16], lo[16];
-    load8(x + i0, hi, vec);
-    load8(x + i0 + 8, hi + 8, vec);
-#pragma unroll
-    for (int i = 0; i < 16; ++i) lo[i] = 0.f;
-    if (rotate && kind != 2) {
-      float y[16];  // partners
-      if (a.interleaved) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) y[i] = hi[i ^ 1];
-      } else if (blocks) {
-#pragma unroll
-        for (int b = 0; b < 16; b += 8) {
-          const int dim = i0 + b;
-          load8(x + (dim < half ? dim + half : dim < a.rotary ? dim - half : dim), y + b, vec);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int dim = i0 + i;
-          y[i] = to_f32(x[dim < half ? dim + half : dim < a.rotary ? dim - half : dim]);
-        }
-      }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        if (i0 + i >= a.rotary) continue;
-        if (kind == 1) {
-          rotate_pair(hi[i], c[i], y[i], s[i], hi[i], lo[i]);
-        } else {
-          hi[i] = fmaf(hi[i], c[i], y[i] * s[i]);
-        }
-      }
-    }
-    if (kind == 0) {
-      // q_out may be q: the head's threads (one warp's) have read their partners
-      __syncwarp(((1u << groups) - 1u) << ((threadIdx.x & 31) / groups * groups));
-      TQ* o = static_cast<TQ*>(a.q_out) + row * a.qo_row + g * a.qo_head + i0;
-      store8(o, hi, ovec);
-      store8(o + 8, hi + 8, ovec);
-      continue;
-    }
-    uint8_t* page = kv4_page(a.c, sid, pos, g);
-    if (page == nullptr) continue;
-    const int r = pos % kKv4Page;
-    uint2 codes;
-    const uint32_t b = kv4_quantise(hi, lo, codes);
-    if (kind == 1) {
-      *reinterpret_cast<uint2*>(page + kv4_k_code(grp, r)) = codes;
-      page[kv4_k_scale(a.c.d, grp, r)] = static_cast<uint8_t>(b);
-    } else {
-      const uint32_t w[4] = {codes.x & 0xFFFFu, codes.x >> 16, codes.y & 0xFFFFu, codes.y >> 16};
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<uint16_t*>(page + kv4_v_code(a.c.d, 4 * grp + i, r)) = static_cast<uint16_t>(w[i]);
-      page[kv4_v_scale(a.c.d, grp, r)] = static_cast<uint8_t>(b);
-    }
-  }
-}
-
-// ---- read --------------------------------------------------------------------------
-// Rows out of the cache as values (zeros where the position is negative or the
-// table names no page).  Thread = (row, kv head, K or V, group).
-template <class T>
-__global__ void __launch_bounds__(256) kv4_read_kernel(const __grid_constant__ Kv4ReadArgs a) {
-  const int groups = a.c.d >> 4;
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t per_row = static_cast<int64_t>(a.c.n_kv) * 2 * groups;
-  if (i >= a.n_rows * per_row) return;
-  const int row = static_cast<int>(i / per_row), rest = static_cast<int>(i % per_row);
-  const int g = rest / (2 * groups), kv = rest / groups % 2, grp = rest % groups;
-  const int pos = a.pos[row];
-  const uint8_t* page = nullptr;
-  if (pos >= 0) page = kv4_page(a.c, a.seq != nullptr ? a.seq[row] : row, pos, g);
-  float x[16];
-#pragma unroll
-  for (int k = 0; k < 16; ++k) x[k] = 0.f;
-  if (page != nullptr) {
-    const int r = pos % kKv4Page;
-    uint2 codes;
-    uint32_t b;
-    if (kv == 0) {
-      codes = *reinterpret_cast<const uint2*>(page + kv4_k_code(grp, r));
-      b = page[kv4_k_scale(a.c.d, grp, r)];
-    } else {
-      uint32_t w[4];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) w[k] = *reinterpret_cast<const uint16_t*>(page + kv4_v_code(a.c.d, 4 * grp + k, r));
-      codes = make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-      b = page[kv4_v_scale(a.c.d, grp, r)];
-    }
-    const float s = kv4_scale_value(b);
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      x[k] = s * static_cast<float>(static_cast<int>((codes.x >> (4 * k)) & 15u) - 8);
-      x[8 + k] = s * static_cast<float>(static_cast<int>((codes.y >> (4 * k)) & 15u) - 8);
-    }
-  }
-  T* o = static_cast<T*>(kv == 0 ? a.k : a.v) + (static_cast<int64_t>(row) * a.c.n_kv + g) * a.c.d + grp * 16;
-  const bool vec = (reinterpret_cast<uintptr_t>(o) & 15u) == 0;
-  store8(o, x, vec);
-  store8(o + 8, x + 8, vec);
-}
-
-// ---- attention -----------------------------------------------------------------------
-// S^T = K Q^T and O^T = V^T P^T on m16n8k16 in half: the 16 positions of a page
-// are the rows of the first product and the reduction of the second, the query
-// columns (row of the sequence, head of the group) its 8 columns, so no
-// fragment of the cache is wasted on absent queries.
-//
-// Both operands of both products are exact but for the probabilities: held
-// values are halves, half queries are taken as they are, and bf16 queries (8
-// significant bits) become halves after each column is divided by the power of
-// two below its largest magnitude, which the softmax scale takes back; what
-// that loses of dims 2^28 times smaller than the largest is far below a
-// float32 sum's own rounding.  Probabilities keep 11 bits: they carry a factor
-// 2^15, so those down to 2^-29 of the row's largest are normal halves, and the
-// sum they are divided by carries it too.
-constexpr float kKv4POffset = 15.f;
-
-// Four halves-pairs of a code word: nibbles (i, i + 4) for i = 0 .. 3, each
+// Four pairs of halves of a code word: nibbles (i, i + 4) for i = 0 .. 3, each
 // times its scale.  1024 + u (bits 0-3 of a half's mantissa) less 1032, or
 // 1024 + 16 u (bits 4-7) over 16 less 72, is u - 8 exactly; so is the product.
 __device__ __forceinline__ void kv4_values(uint32_t w, uint32_t s, uint32_t (&v)[4]) {
@@ -385,6 +266,264 @@ __device__ __forceinline__ void kv4_values(uint32_t w, uint32_t s, uint32_t (&v)
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
       : "r"(w), "r"(x), "r"(s), "r"(0x64086408u), "r"(0x2C002C00u), "r"(0xD480D480u));
 }
+
+// ---- append ------------------------------------------------------------------------
+// Thread = (8 dims, slice of the heads): a block on one row, d / 8 octets by its
+// other threads' slices; a thread keeps its 8 dims' angles in registers over
+// the heads it walks.  Reads and writes of rows are 16 bytes a lane, contiguous
+// over a head.  blockIdx.x = row; gridDim.y = 1: a block takes the whole row;
+// else blockIdx.y = a batch of query heads, one a thread, then K, then V.
+// 10242 rows of 32 + 8 + 8 heads of 128 (252 MB with the read-back): 80 us, and
+// 18 us to read the rows back; the instructions of the rotation and of deciding
+// codes bound it (2 a cycle and SM), not memory, whose share is 36 us.
+constexpr int kKv4AppendThreads = 128;  // at most; one warp a row where there are many rows (see kv4.cu)
+
+// How the first `rotary` dims of a head pair up.
+enum Kv4Rope { kRopeNone, kRopeBlocks, kRopePairs, kRopeAny };  // none; i, i + half with half % 8 = 0; 2i, 2i + 1; else
+
+// The angles of a thread's 8 dims from i0: out[i] = x[i] c[i] + partner[i] s[i].
+template <int ROPE>
+__device__ __forceinline__ void kv4_angles(const Kv4AppendArgs& a, int pos, int i0, float (&c)[8], float (&s)[8]) {
+  const int half = a.rotary >> 1;
+  const float* cr = a.cos + static_cast<int64_t>(pos) * half;
+  const float* sr = a.sin + static_cast<int64_t>(pos) * half;
+  const bool vec = ((reinterpret_cast<uintptr_t>(cr) | reinterpret_cast<uintptr_t>(sr)) & 15u) == 0;
+  if (ROPE == kRopeBlocks && vec) {
+    const int f = i0 < half ? i0 : i0 - half;
+    const float sign = i0 < half ? -1.f : 1.f;
+#pragma unroll
+    for (int k = 0; k < 2; ++k) {
+      const float4 x = __ldg(reinterpret_cast<const float4*>(cr + f) + k), y = __ldg(reinterpret_cast<const float4*>(sr + f) + k);
+      c[4 * k] = x.x; c[4 * k + 1] = x.y; c[4 * k + 2] = x.z; c[4 * k + 3] = x.w;
+      s[4 * k] = sign * y.x; s[4 * k + 1] = sign * y.y; s[4 * k + 2] = sign * y.z; s[4 * k + 3] = sign * y.w;
+    }
+  } else if (ROPE == kRopePairs && vec && (half & 3) == 0) {
+    const float4 x = __ldg(reinterpret_cast<const float4*>(cr + (i0 >> 1))), y = __ldg(reinterpret_cast<const float4*>(sr + (i0 >> 1)));
+    c[0] = c[1] = x.x; c[2] = c[3] = x.y; c[4] = c[5] = x.z; c[6] = c[7] = x.w;
+    s[0] = -y.x; s[1] = y.x; s[2] = -y.y; s[3] = y.y;
+    s[4] = -y.z; s[5] = y.z; s[6] = -y.w; s[7] = y.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int dim = i0 + i;
+      c[i] = 1.f;
+      s[i] = 0.f;
+      if (dim < a.rotary) {
+        const int f = ROPE == kRopePairs ? dim >> 1 : dim < half ? dim : dim - half;
+        const bool first = ROPE == kRopePairs ? (dim & 1) == 0 : dim < half;
+        c[i] = __ldg(cr + f);
+        s[i] = first ? -__ldg(sr + f) : __ldg(sr + f);
+      }
+    }
+  }
+}
+// The partners of a head's 8 dims from i0, where they are elsewhere in the head.
+template <int ROPE, class T>
+__device__ __forceinline__ Eight<T> kv4_partners(const Kv4AppendArgs& a, const T* head, int i0, bool vec) {
+  const int half = a.rotary >> 1;
+  if (ROPE == kRopeBlocks) return load8(head + (i0 < half ? i0 + half : i0 - half), vec);
+  Eight<T> y;
+  if (ROPE == kRopeAny) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int dim = i0 + i;
+      y.v[i] = head[dim < half ? dim + half : dim < a.rotary ? dim - half : dim];
+    }
+  }
+  return y;
+}
+
+template <class T, class TQ, int ROPE>
+__global__ void __launch_bounds__(kKv4AppendThreads, 6) kv4_append_kernel(
+    const __grid_constant__ Kv4AppendArgs a) {
+  pdl_wait();
+  pdl_launch();
+  const int oct_bits = a.c.d == 64 ? 3 : 4;  // d / 8 octets
+  const int oct = threadIdx.x & ((1 << oct_bits) - 1), slice = threadIdx.x >> oct_bits, slices = blockDim.x >> oct_bits;
+  const int64_t row = blockIdx.x;
+  const int i0 = oct * 8, y = blockIdx.y;
+  const int nq = a.q != nullptr ? a.n_heads : 0, q_batches = gridDim.y - 2;
+  const bool all = gridDim.y == 1, do_k = all || y == q_batches, do_v = all || y == q_batches + 1;
+  const bool turns = ROPE != kRopeNone && i0 < a.rotary;  // some of the thread's dims turn
+  const bool part = ROPE != kRopeNone && i0 + 8 > a.rotary;  // but not all of them
+  const bool kvec = aligned16(a.k, a.k_row, a.k_head, sizeof(T)), vvec = aligned16(a.v, a.v_row, a.v_head, sizeof(T));
+  const int pos = __ldg(a.pos + row);
+  const int sid = a.seq != nullptr ? __ldg(a.seq + row) : static_cast<int>(row);
+  // Loops below are alike for all threads of the block (a thread without a head
+  // goes along): the warp stays together.
+  const T* k = static_cast<const T*>(a.k) + row * a.k_row + slice * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + row * a.v_row + slice * a.v_head;
+  Eight<T> kx = {}, ky = {}, vx = {};
+  auto fetch_k = [&](int g) {
+    if (g < a.c.n_kv) {
+      kx = load8(k + i0, kvec);
+      if (turns) ky = kv4_partners<ROPE>(a, k, i0, kvec);
+    }
+  };
+  if (do_k) fetch_k(slice);
+  if (do_v && slice < a.c.n_kv) vx = load8(v + i0, vvec);
+  if (pos < 0) return;  // idle row
+  if (ROPE != kRopeNone && pos >= a.max_pos) {
+    if (threadIdx.x == 0) kv4_error(a.c.status, kKv4BadPos);
+    return;
+  }
+  float c[8], s[8];
+  if (turns) kv4_angles<ROPE>(a, pos, i0, c, s);
+
+  if (all || y < q_batches) {
+    const bool qvec = aligned16(a.q, a.q_row, a.q_head, sizeof(T)), ovec = aligned16(a.q_out, a.qo_row, a.qo_head, sizeof(TQ));
+    const int h0 = all ? 0 : y * slices, h1 = all ? nq : min(nq, (y + 1) * slices);
+    const T* q = static_cast<const T*>(a.q) + row * a.q_row + (h0 + slice) * a.q_head;
+    TQ* o = static_cast<TQ*>(a.q_out) + row * a.qo_row + (h0 + slice) * a.qo_head + i0;
+    const int64_t q_step = slices * a.q_head, o_step = slices * a.qo_head;
+#pragma unroll 2
+    for (int h = h0; h < h1; h += slices, q += q_step, o += o_step) {
+      const bool mine = h + slice < h1;
+      Eight<T> x = {}, p = {};
+      if (mine) {
+        x = load8(q + i0, qvec);
+        if (turns) p = kv4_partners<ROPE>(a, q, i0, qvec);
+      }
+      float r[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = to_f32(x.v[i]);
+      if (turns) {
+        float z[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = ROPE == kRopePairs ? r[i ^ 1] : to_f32(p.v[i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = fmaf(r[i], c[i], z[i] * s[i]);
+        if (part) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i0 + i >= a.rotary) r[i] = to_f32(x.v[i]);
+        }
+      }
+      __syncwarp();  // q_out may be q: a head's threads, all of one warp, have read their partners
+      if (mine) store8(o, r, ovec);
+    }
+  }
+  if (!do_k && !do_v) return;
+  uint8_t* page = kv4_page(a.c, sid, pos, slice);
+  if (page == nullptr) return;
+  const int r = pos % kKv4Page, page_step = slices * kv4_page_bytes(a.c.d);
+  if (do_k) {
+    const int code_at = kv4_k_code(oct >> 1, r) + 4 * (oct & 1), scale_at = kv4_k_scale(a.c.d, oct >> 1, r);
+    const bool few = sizeof(T) == 2 && !(ROPE != kRopeNone && (i0 & ~15) < a.rotary);  // (alike over a group)
+    uint8_t* to = page;
+    for (int g = slice; g - slice < a.c.n_kv; g += slices, to += page_step) {
+      float hi[8], lo[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        hi[i] = to_f32(kx.v[i]);
+        lo[i] = 0.f;
+      }
+      if (turns) {
+        float z[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = ROPE == kRopePairs ? hi[i ^ 1] : to_f32(ky.v[i]);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) rotate_pair(hi[i], c[i], z[i], s[i], hi[i], lo[i]);
+        if (part) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i0 + i >= a.rotary) {
+              hi[i] = to_f32(kx.v[i]);
+              lo[i] = 0.f;
+            }
+        }
+      }
+      k += slices * a.k_head;
+      fetch_k(g + slices);
+      uint32_t codes;
+      const uint32_t b = kv4_quantise(hi, lo, few, codes);
+      if (g < a.c.n_kv) {
+        *reinterpret_cast<uint32_t*>(to + code_at) = codes;
+        if ((oct & 1) == 0) to[scale_at] = static_cast<uint8_t>(b);
+      }
+    }
+  }
+  if (do_v) {
+    const int code_at = kv4_v_code(a.c.d, 2 * oct, r), scale_at = kv4_v_scale(a.c.d, oct >> 1, r);
+    for (int g = slice; g - slice < a.c.n_kv; g += slices, page += page_step) {
+      float hi[8], lo[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        hi[i] = to_f32(vx.v[i]);
+        lo[i] = 0.f;
+      }
+      v += slices * a.v_head;
+      if (g + slices < a.c.n_kv) vx = load8(v + i0, vvec);
+      uint32_t codes;
+      const uint32_t b = kv4_quantise(hi, lo, sizeof(T) == 2, codes);
+      if (g < a.c.n_kv) {
+        uint16_t* to = reinterpret_cast<uint16_t*>(page + code_at);
+        to[0] = static_cast<uint16_t>(codes);
+        to[2] = static_cast<uint16_t>(codes >> 16);  // (the next quad's two bytes are 4 bytes on)
+        if ((oct & 1) == 0) page[scale_at] = static_cast<uint8_t>(b);
+      }
+    }
+  }
+}
+
+// ---- read --------------------------------------------------------------------------
+// Rows out of the cache as values (zeros where the position is negative or the
+// table names no page).  Block: 128 threads on one row; thread = 8 dims of a
+// kv head's K or V.
+template <class T>
+__global__ void __launch_bounds__(128) kv4_read_kernel(const __grid_constant__ Kv4ReadArgs a) {
+  pdl_wait();
+  pdl_launch();
+  const int octs = a.c.d >> 3, oct = threadIdx.x & (octs - 1);
+  const int64_t row = blockIdx.x;
+  const int pos = __ldg(a.pos + row), sid = a.seq != nullptr ? __ldg(a.seq + row) : static_cast<int>(row);
+  const uint8_t* block = pos >= 0 ? kv4_page(a.c, sid, pos, 0) : nullptr;
+  const int r = pos >= 0 ? pos % kKv4Page : 0, step = 128 / octs * gridDim.y;
+  const bool kvec = (reinterpret_cast<uintptr_t>(a.k) & 15u) == 0, vvec = (reinterpret_cast<uintptr_t>(a.v) & 15u) == 0;
+#pragma unroll 4
+  for (int hh = threadIdx.x / octs + blockIdx.y * (128 / octs); hh < 2 * a.c.n_kv; hh += step) {
+    const bool is_k = hh < a.c.n_kv;
+    const int g = is_k ? hh : hh - a.c.n_kv;
+    uint32_t p[4] = {0u, 0u, 0u, 0u};  // dims (0, 1), (2, 3), ..
+    if (block != nullptr) {
+      const uint8_t* page = block + g * kv4_page_bytes(a.c.d);
+      uint32_t codes, b;
+      if (is_k) {
+        codes = *reinterpret_cast<const uint32_t*>(page + kv4_k_code(oct >> 1, r) + 4 * (oct & 1));
+        b = page[kv4_k_scale(a.c.d, oct >> 1, r)];
+      } else {
+        const uint16_t* w = reinterpret_cast<const uint16_t*>(page + kv4_v_code(a.c.d, 2 * oct, r));
+        codes = w[0] | (static_cast<uint32_t>(w[2]) << 16);  // (the next quad's two bytes are 4 bytes on)
+        b = page[kv4_v_scale(a.c.d, oct >> 1, r)];
+      }
+      uint32_t v[4];
+      kv4_values(codes, b * 0x00800080u, v);
+      p[0] = __byte_perm(v[0], v[1], 0x5410);
+      p[1] = __byte_perm(v[2], v[3], 0x5410);
+      p[2] = __byte_perm(v[0], v[1], 0x7632);
+      p[3] = __byte_perm(v[2], v[3], 0x7632);
+    }
+    T* out = static_cast<T*>(is_k ? a.k : a.v) + (row * a.c.n_kv + g) * a.c.d + 8 * oct;
+    put8(out, p, is_k ? kvec : vvec);
+  }
+}
+
+// ---- attention -----------------------------------------------------------------------
+// S^T = K Q^T and O^T = V^T P^T on m16n8k16 in half: the 16 positions of a page
+// are the rows of the first product and the reduction of the second, the query
+// columns (row of the sequence, head of the group) its 8 columns, so no
+// fragment of the cache is wasted on absent queries.
+//
+// Both operands of both products are exact but for the probabilities: held
+// values are halves, half queries are taken as they are, and bf16 queries (8
+// significant bits) become halves after each column is divided by the power of
+// two below its largest magnitude, which the softmax scale takes back; what
+// that loses of dims 2^28 times smaller than the largest is far below a
+// float32 sum's own rounding.  Probabilities keep 11 bits: they carry a factor
+// 2^15, so those down to 2^-29 of the row's largest are normal halves, and the
+// sum they are divided by carries it too.
+constexpr float kKv4POffset = 15.f;
+
 // Scale pair from two bytes of w: selector 0x4i4j puts bytes j, i into the halves.
 __device__ __forceinline__ uint32_t kv4_scales(uint32_t w, uint32_t selector) {
   return __byte_perm(w, 0u, selector) * 128u;
@@ -537,10 +676,11 @@ __device__ __forceinline__ float* kv4_part(const Kv4AttnArgs& a, int seq, int g,
 constexpr int kKv4Ahead = 2;
 constexpr uint64_t kKv4WaitNs = 200000000ull;  // bound on every page wait
 constexpr __host__ __device__ int kv4_step_pages(int nh) { return nh == 1 ? 4 : 2; }
-template <int NH, int NB, int W>
+constexpr int kKv4Warps = 4;  // of a CTA (2: the same on a wave of 256; 1: slower everywhere)
+template <int NH, int NB>
 constexpr __host__ __device__ int kv4_attn_smem() {
-  constexpr int ring = W * (kKv4Ahead + 1) * kv4_step_pages(NH) * kv4_page_bytes(64 * NH);
-  constexpr int join = W == 1 ? 0 : W * 8 * NB * (64 * NH + 2) * 4;  // reuses the ring
+  constexpr int W = kKv4Warps, ring = W * (kKv4Ahead + 1) * kv4_step_pages(NH) * kv4_page_bytes(64 * NH);
+  constexpr int join = W * 8 * NB * (64 * NH + 2) * 4;  // reuses the ring
   return ring > join ? ring : join;
 }
 
@@ -550,9 +690,9 @@ constexpr __host__ __device__ int kv4_attn_smem() {
 // A page's bytes are contiguous: each comes by one bulk copy into the warp's
 // ring, kKv4Ahead steps ahead; a step takes P pages, so the running maximum
 // and the rescaling of o are paid once for 16 P positions.
-template <class T, int NH, int NB, int W>
-__global__ void __launch_bounds__(32 * W) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
-  constexpr int D = 64 * NH, COLS = 8 * NB, P = kv4_step_pages(NH), PB = kv4_page_bytes(D), SLOTS = kKv4Ahead + 1;
+template <class T, int NH, int NB>
+__global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
+  constexpr int W = kKv4Warps, D = 64 * NH, COLS = 8 * NB, P = kv4_step_pages(NH), PB = kv4_page_bytes(D), SLOTS = kKv4Ahead + 1;
   extern __shared__ __align__(16) uint8_t kv4_smem[];
   __shared__ uint64_t s_bar[W][SLOTS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gid = lane >> 2, tig = lane & 3;
@@ -822,26 +962,6 @@ __global__ void __launch_bounds__(32 * W) kv4_attn_kernel(const __grid_constant_
       if (d0 == 0) *reinterpret_cast<float2*>(dst + D) = make_float2(M, L);
     }
   };
-  if constexpr (W == 1) {
-#pragma unroll
-    for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int c = c0 + 8 * nb + 2 * tig + e;
-        if (c >= cols) continue;
-#pragma unroll
-        for (int h = 0; h < NH; ++h) {
-          float r[8];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            r[2 * j] = o[nb][4 * h + j][e];
-            r[2 * j + 1] = o[nb][4 * h + j][2 + e];
-          }
-          put(c, 64 * h + 8 * gid, r, m[nb][e] * up[nb][e], l[nb][e]);
-        }
-      }
-    return;
-  }
   __syncthreads();  // the ring's memory becomes the warps' states
   float(*s_o)[COLS][D] = reinterpret_cast<float(*)[COLS][D]>(kv4_smem);
   float(*s_m)[COLS] = reinterpret_cast<float(*)[COLS]>(kv4_smem + sizeof(float) * W * COLS * D);

@@ -58,7 +58,6 @@ struct Kv4AttnArgs {
   // set by kv4_attn_plan: query columns (row, head) per tile, tiles per
   // (sequence, kv head), splits of the positions and pages per split
   int tile_cols, tiles, splits, split_pages;
-  int warps;               // of a CTA (1, 2 or 4)
   int group;               // query heads of a kv head
   uint64_t group_inv;      // ceil(2^32 / group): c / group = c * group_inv >> 32 while c * group < 2^32
 };
