@@ -97,12 +97,12 @@ def attention_bound(out, mass, size, length, d, half_step, vmax):
     * float32 sums over the positions: a chain of length / 16 products of 16
       and the rescaling after each, (length / 16 + 64) 2^-23 of sum p |v|,
       again for numerator and divisor;
-    * a probability is a half with a factor of 2^15 that the row's sum (at least
-      that factor) carries too; halves below 2^-14 are 2^-24 apart, so it is off
-      by up to 2^-25 / 2^15 = 2^-40, at each of `length` positions with
+    * a probability is a half with a factor of at least 2^10 that the row's sum
+      (at least that factor) carries too; halves below 2^-14 are 2^-24 apart, so
+      it is off by up to 2^-25 / 2^10 = 2^-35, at each of `length` positions with
       |v| <= vmax;
     * an fp16 result's rounding is off by up to 2^-25 however small it is.
     """
-    low = length * 2.0 ** -40 * vmax + (2.0 ** -25 if half_step == 2.0 ** -11 else 0.0)
+    low = length * 2.0 ** -35 * vmax + (2.0 ** -25 if half_step == 2.0 ** -11 else 0.0)
     share = 2.0 ** -11 + 4 * (d + 6) * 2.0 ** -24 * size + 2.0 ** -20 + 2 * (length / 16 + 64) * 2.0 ** -23
     return half_step * np.abs(out) + share * (1 + half_step) * mass + low + 1e-30

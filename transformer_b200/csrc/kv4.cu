@@ -3,10 +3,12 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 
 #include "b2d_host.h"
 #include "kv4.cuh"
+#include "kv4_prompt.cuh"
 
 namespace b2d {
 
@@ -42,22 +44,38 @@ cudaError_t raise_smem() {
   return e;
 }
 
+template <class T, int NH>
+cudaError_t join(const Kv4AttnArgs& a, cudaStream_t st) {
+  if (a.splits == 1) return cudaSuccess;
+  return launch(kv4_join_kernel<T, NH>,
+                dim3(static_cast<unsigned>(a.n_seqs), static_cast<unsigned>(a.c.n_kv),
+                     static_cast<unsigned>(a.max_rows * a.group)),
+                dim3(128), 0, st, true, a);
+}
+
+template <auto Kernel, int Smem, class T, int NH>
+cudaError_t launch_tiles(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
+  cudaError_t e = raise_smem<Kernel, Smem>();
+  if (e == cudaSuccess)
+    e = launch(Kernel,
+               dim3(static_cast<unsigned>(a.n_seqs), static_cast<unsigned>(a.c.n_kv),
+                    static_cast<unsigned>(a.tiles * a.splits)),
+               dim3(128), Smem, st, pdl, a);
+  return e == cudaSuccess ? join<T, NH>(a, st) : e;
+}
 template <class T, int NH, int NB>
 cudaError_t attn_launch(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
-  constexpr int smem = kv4_attn_smem<NH, NB>();
-  cudaError_t e = raise_smem<kv4_attn_kernel<T, NH, NB>, smem>();
-  const unsigned x = static_cast<unsigned>(a.n_seqs), y = static_cast<unsigned>(a.c.n_kv);
-  if (e == cudaSuccess)
-    e = launch(kv4_attn_kernel<T, NH, NB>, dim3(x, y, static_cast<unsigned>(a.tiles * a.splits)), dim3(32 * kKv4Warps), smem,
-               st, pdl, a);
-  if (e == cudaSuccess && a.splits > 1)
-    e = launch(kv4_join_kernel<T, NH>, dim3(x, y, static_cast<unsigned>(a.max_rows * a.group)), dim3(128), 0, st, true,
-               a);
-  return e;
+  static_assert(32 * kKv4Warps == 128, "block of launch_tiles");
+  return launch_tiles<kv4_attn_kernel<T, NH, NB>, kv4_attn_smem<NH, NB>(), T, NH>(a, st, pdl);
+}
+template <class T, int NH>
+cudaError_t prompt_launch(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
+  return launch_tiles<kv4_prompt_kernel<T, NH>, kv4_prompt_smem<NH>(), T, NH>(a, st, pdl);
 }
 
 template <class T, int NH>
 cudaError_t attn_shape(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
+  if (a.tile_cols == kKv4PromptCols) return prompt_launch<T, NH>(a, st, pdl);
   return a.tile_cols > 8 ? attn_launch<T, NH, 2>(a, st, pdl) : attn_launch<T, NH, 1>(a, st, pdl);
 }
 
@@ -95,7 +113,8 @@ bool kv4_attn_plan(Kv4AttnArgs& a, int sms) {
   a.group_inv = ((uint64_t(1) << 32) + a.group - 1) / a.group;
   const int64_t cols = static_cast<int64_t>(a.max_rows) * a.group;
   if (cols * a.group >= int64_t(1) << 32) return false;
-  a.tile_cols = cols <= 8 ? 8 : 16;
+  static const int thr = getenv("KV4_THR") ? atoi(getenv("KV4_THR")) : 32;
+  a.tile_cols = cols <= 8 ? 8 : cols <= thr ? 16 : kKv4PromptCols;
   a.tiles = static_cast<int>((cols + a.tile_cols - 1) / a.tile_cols);
   const int pages = std::max(1, (a.max_len + kKv4Page - 1) / kKv4Page);
   const int64_t units = static_cast<int64_t>(a.n_seqs) * a.c.n_kv * a.tiles;
@@ -103,8 +122,9 @@ bool kv4_attn_plan(Kv4AttnArgs& a, int sms) {
   // one wave of CTAs, four to an SM (131071 positions, 8 kv heads of 128: 45 us,
   // and 55 us with splits for four waves).  Several sequences differ in length:
   // four waves even that out (32 of 1001 to 16384: 93 us, and 110 us with one).
-  const int64_t ctas = int64_t(sms) * (a.n_seqs == 1 ? 4 : 16);
-  const int64_t splits = std::max<int64_t>(1, std::min<int64_t>(ctas / std::max<int64_t>(1, units), (pages + 31) / 32));
+  const bool prompt = a.tile_cols == kKv4PromptCols;
+  const int64_t ctas = int64_t(sms) * (prompt ? 2 : a.n_seqs == 1 ? 4 : 16);
+  const int64_t splits = prompt ? std::max<int64_t>(1, std::min<int64_t>(ctas / std::max<int64_t>(1, units), pages / 64)) : std::max<int64_t>(1, std::min<int64_t>(ctas / std::max<int64_t>(1, units), (pages + 31) / 32));
   a.split_pages = static_cast<int>((pages + splits - 1) / splits);
   a.splits = (pages + a.split_pages - 1) / a.split_pages;
   // the grid's y and z
