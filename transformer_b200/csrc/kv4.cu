@@ -3,7 +3,6 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
-#include <cstdlib>
 #include <cstring>
 
 #include "b2d_host.h"
@@ -53,24 +52,23 @@ cudaError_t join(const Kv4AttnArgs& a, cudaStream_t st) {
                 dim3(128), 0, st, true, a);
 }
 
-template <auto Kernel, int Smem, class T, int NH>
+template <auto Kernel, int Threads, int Smem, class T, int NH>
 cudaError_t launch_tiles(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
   cudaError_t e = raise_smem<Kernel, Smem>();
   if (e == cudaSuccess)
     e = launch(Kernel,
                dim3(static_cast<unsigned>(a.n_seqs), static_cast<unsigned>(a.c.n_kv),
                     static_cast<unsigned>(a.tiles * a.splits)),
-               dim3(128), Smem, st, pdl, a);
+               dim3(Threads), Smem, st, pdl, a);
   return e == cudaSuccess ? join<T, NH>(a, st) : e;
 }
 template <class T, int NH, int NB>
 cudaError_t attn_launch(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
-  static_assert(32 * kKv4Warps == 128, "block of launch_tiles");
-  return launch_tiles<kv4_attn_kernel<T, NH, NB>, kv4_attn_smem<NH, NB>(), T, NH>(a, st, pdl);
+  return launch_tiles<kv4_attn_kernel<T, NH, NB>, 32 * kKv4Warps, kv4_attn_smem<NH, NB>(), T, NH>(a, st, pdl);
 }
 template <class T, int NH>
 cudaError_t prompt_launch(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
-  return launch_tiles<kv4_prompt_kernel<T, NH>, kv4_prompt_smem<NH>(), T, NH>(a, st, pdl);
+  return launch_tiles<kv4_prompt_kernel<T, NH>, kKv4PromptThreads, kv4_prompt_smem<NH>(), T, NH>(a, st, pdl);
 }
 
 template <class T, int NH>
@@ -113,8 +111,10 @@ bool kv4_attn_plan(Kv4AttnArgs& a, int sms) {
   a.group_inv = ((uint64_t(1) << 32) + a.group - 1) / a.group;
   const int64_t cols = static_cast<int64_t>(a.max_rows) * a.group;
   if (cols * a.group >= int64_t(1) << 32) return false;
-  static const int thr = getenv("KV4_THR") ? atoi(getenv("KV4_THR")) : 32;
-  a.tile_cols = cols <= 8 ? 8 : cols <= thr ? 16 : kKv4PromptCols;
+  // The kernel for prompts takes 128 columns at the price of any: from 65 columns
+  // (16 rows of 4 heads and 128 dims on 2048 positions, 8 sequences: 31 us, and
+  // 40 with tiles of 16; at 64 dims 24 and 17; 32 rows on 8000: 27 and 34).
+  a.tile_cols = cols <= 8 ? 8 : cols <= 64 ? 16 : kKv4PromptCols;
   a.tiles = static_cast<int>((cols + a.tile_cols - 1) / a.tile_cols);
   const int pages = std::max(1, (a.max_len + kKv4Page - 1) / kKv4Page);
   const int64_t units = static_cast<int64_t>(a.n_seqs) * a.c.n_kv * a.tiles;
@@ -122,9 +122,12 @@ bool kv4_attn_plan(Kv4AttnArgs& a, int sms) {
   // one wave of CTAs, four to an SM (131071 positions, 8 kv heads of 128: 45 us,
   // and 55 us with splits for four waves).  Several sequences differ in length:
   // four waves even that out (32 of 1001 to 16384: 93 us, and 110 us with one).
+  // Prompts: only where the tiles leave CTA slots empty, 64 pages each at least
+  // (the join reads and writes every column's share: 274 us became 364).
   const bool prompt = a.tile_cols == kKv4PromptCols;
-  const int64_t ctas = int64_t(sms) * (prompt ? 2 : a.n_seqs == 1 ? 4 : 16);
-  const int64_t splits = prompt ? std::max<int64_t>(1, std::min<int64_t>(ctas / std::max<int64_t>(1, units), pages / 64)) : std::max<int64_t>(1, std::min<int64_t>(ctas / std::max<int64_t>(1, units), (pages + 31) / 32));
+  const int64_t ctas = int64_t(sms) * (prompt ? 2 : a.n_seqs == 1 ? 4 : 16), least = prompt ? 64 : 32;
+  const int64_t splits =
+      std::max<int64_t>(1, std::min<int64_t>(ctas / std::max<int64_t>(1, units), (pages + least - 1) / least));
   a.split_pages = static_cast<int>((pages + splits - 1) / splits);
   a.splits = (pages + a.split_pages - 1) / a.split_pages;
   // the grid's y and z

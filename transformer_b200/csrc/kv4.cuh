@@ -672,9 +672,38 @@ __device__ __forceinline__ float* kv4_part(const Kv4AttnArgs& a, int seq, int g,
   return a.part + ((unit * a.splits + split) * a.tile_cols + col) * (d + 4);
 }
 
+// Waits for a phase of an mbarrier: tries that sleep up to a microsecond each,
+// at most kKv4Tries of them (0.2 s).  No timer and no call: either one in the
+// loop made the compiler spill around every wait.
+constexpr uint32_t kKv4Tries = 200000u;
+__device__ __forceinline__ bool kv4_wait(uint64_t* bar, uint32_t parity) {
+  const uint32_t at = smem_addr(bar);
+  uint32_t ok = 0u;
+  for (uint32_t i = 0; i < kKv4Tries && !ok; ++i)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(at), "r"(parity), "r"(1000u) : "memory");
+  return ok != 0u;
+}
+// The same without sleeping, for a warp that others wait for (a sleeping one was
+// seen to wake up some 250 cycles late).
+constexpr uint32_t kKv4Polls = 1u << 23;
+__device__ __forceinline__ bool kv4_poll(uint64_t* bar, uint32_t parity) {
+  const uint32_t at = smem_addr(bar);
+  uint32_t ok = 0u;
+  for (uint32_t i = 0; i < kKv4Polls && !ok; ++i)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.acquire.cta.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok) : "r"(at), "r"(parity) : "memory");
+  return ok != 0u;
+}
+
 // The pages of a warp's ring: kKv4Ahead + 1 steps of P pages.
 constexpr int kKv4Ahead = 2;
-constexpr uint64_t kKv4WaitNs = 200000000ull;  // bound on every page wait
 constexpr __host__ __device__ int kv4_step_pages(int nh) { return nh == 1 ? 4 : 2; }
 constexpr int kKv4Warps = 4;  // of a CTA (2: the same on a wave of 256; 1: slower everywhere)
 template <int NH, int NB>
@@ -747,13 +776,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
     uint64_t* b = &bar[slot];
     const uint32_t parity = (phase >> slot) & 1u;
     phase ^= 1u << slot;
-    if (mbar_test(b, parity)) return;
-    const uint64_t t0 = globaltimer_ns();
-    for (uint32_t i = 1; !mbar_test(b, parity); ++i)
-      if ((i & 255u) == 0 && globaltimer_ns() - t0 > kKv4WaitNs) {
-        waited = false;
-        return;
-      }
+    if (!kv4_wait(b, parity)) waited = false;
   };
   int id = load_id(0);
 #pragma unroll
