@@ -130,6 +130,12 @@ B2D_API int b2d_model_grid(const b2d_model* m);
  * nothing is allocated per step.  One workspace per stream; not re-entrant. */
 B2D_API b2d_status b2d_workspace_create(b2d_model* m, int max_batch, b2d_ws** out);
 B2D_API b2d_status b2d_workspace_destroy(b2d_ws* ws);
+/* What the paged pools given with this workspace hold: bits 16 (default), bf16
+ * values as b2d_decode_step_paged describes; bits 4, the 4-bit format below,
+ * uint8 [n_layers][num_blocks][n_kv_heads][18 * d_head], 16-byte aligned.
+ * b2d_decode_step_paged, b2d_prefill_paged and b2d_prefill_rows follow it.
+ * The first switch to 4 allocates, so it comes before any capture. */
+B2D_API b2d_status b2d_workspace_kv_bits(b2d_ws* ws, int bits);
 /* Clears the exchange words and the device status (after a device error). */
 B2D_API b2d_status b2d_workspace_reset(b2d_ws* ws, void* stream);
 /* Synchronises `stream`, reads the device status word.  Returns B2D_OK or

@@ -166,3 +166,21 @@ def test_held_values_are_exact_in_16_bits():
 def test_held_on_ties_goes_to_even():
     g = np.array([7, 0.5, 1.5, 2.5, -0.5, -1.5, -2.5, 6.5] + [0] * 8, np.float64)
     assert list(R.held(g)[:8]) == [7, 0, 2, 2, 0, -2, -2, 6]
+
+
+def test_submit_refuses_bad_rules():
+    from test_serve_cpu import FakeEngine
+    from transformer_b200.serve import ContinuousBatcher
+    cb = ContinuousBatcher(FakeEngine(), 4, 16)
+    for kw in (dict(presence=float("nan")), dict(frequency=float("inf")), dict(logit_bias={97: 1.0}),
+               dict(logit_bias={-1: 1.0}), dict(logit_bias={3: float("nan")}), dict(allowed=[]), dict(allowed=[97]),
+               dict(allowed=[-1])):
+        with pytest.raises(ValueError):
+            cb.submit([1, 2], 4, **kw)
+    assert cb.idle()
+    rid = cb.submit([1, 2], 4, presence=0.0, frequency=0.0, logit_bias={})
+    assert not cb.waiting[0].rules and cb.waiting[0].greedy and rid == 0
+
+
+def test_workspace_kv_bits_refused(lib):
+    assert lib.b2d_workspace_kv_bits(None, 4) == BAD

@@ -108,6 +108,7 @@ _SIGS = {
     "b2d_model_grid": (ctypes.c_int, [_P]),
     "b2d_workspace_create": (ctypes.c_int, [_P, ctypes.c_int, ctypes.POINTER(_P)]),
     "b2d_workspace_destroy": (ctypes.c_int, [_P]),
+    "b2d_workspace_kv_bits": (ctypes.c_int, [_P, ctypes.c_int]),
     "b2d_workspace_reset": (ctypes.c_int, [_P, _P]),
     "b2d_last_error": (ctypes.c_int, [_P, _P, ctypes.POINTER(ctypes.c_uint32)]),
     "b2d_decode_step": (ctypes.c_int, [_P, _P, _P, _P, ctypes.c_int, _P, _P, _P, _P]),

@@ -19,6 +19,7 @@
 #include "decode_b1.cuh"
 #include "decode_b1c.cuh"
 #include "gemm_tc.cuh"
+#include "kv4.h"
 #include "sampler.cuh"
 
 namespace {
@@ -282,6 +283,11 @@ struct b2d_ws {
   uint32_t tune_gen;       // bumped by every b2d_debug_tune call (cached graphs bake the knobs in)
   bool no_graph;           // step through direct launches only
   cudaStream_t cap_stream; // capture stream (created on first capture)
+  // b2d_workspace_kv_bits: paged pools hold 4 bits a value (kv4.h), else bf16
+  bool kv4;
+  __nv_bfloat16* q4;       // the rows' turned queries [brows][n_heads * 64]
+  float* kv4_part;         // partials of split rows
+  uint64_t kv4_part_bytes;
   // paged attention: TMA view of the last paged pool used (rows of 64 bf16)
   CUtensorMap kvmap;
   const void* kvmap_pool;
@@ -356,6 +362,47 @@ cudaError_t launch_k_smem(void (*k)(KArgs...), dim3 grid, dim3 block, int smem, 
   cfg.attrs = at;
   cfg.numAttrs = pdl ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, k, std::forward<Args>(args)...);
+}
+
+// One layer's 4-bit pool for `batch` rows (table rows table_ld entries apart).
+b2d::Kv4Cache kv4_cache(const b2d_ws* ws, void* pool, const int32_t* table, int table_ld, int bps, int num_blocks,
+                        int batch, int layer) {
+  const b2d_config& c = ws->m->cfg;
+  b2d::Kv4Cache k{};
+  k.pool = static_cast<uint8_t*>(pool) + size_t(layer) * num_blocks * c.n_kv_heads * b2d::kv4_page_bytes(64);
+  k.table = table;
+  k.status = &ws->ctl->status;
+  k.n_kv = c.n_kv_heads;
+  k.d = 64;
+  k.num_blocks = num_blocks;
+  k.bps = bps;
+  k.table_rows = batch;
+  k.table_ld = table_ld;
+  return k;
+}
+// Attention of `batch` rows over it: rows of their own, or (one) of one sequence
+// whose last position is the last row's.
+b2d::Kv4AttnArgs kv4_attn_args(const b2d_ws* ws, const int32_t* pos, const int32_t* table, int table_ld, int bps,
+                               int num_blocks, int batch, bool one, int layer, void* pool = nullptr) {
+  const b2d_config& c = ws->m->cfg;
+  b2d::Kv4AttnArgs a{};
+  a.c = kv4_cache(ws, pool, table, table_ld, bps, num_blocks, batch, layer);
+  a.q = ws->q4;
+  a.out = ws->A;
+  a.q_row = a.o_row = c.d_model;
+  a.q_head = a.o_head = 64;
+  a.lens = one && pos ? pos + batch - 1 : pos;
+  a.len_add = 1;
+  a.part = ws->kv4_part;
+  a.scale_log2 = 0.125f * 1.4426950408889634f;
+  a.n_rows = batch;
+  a.n_heads = c.n_heads;
+  a.n_seqs = one ? 1 : batch;
+  a.max_rows = a.rows_of_one = one ? batch : 0;
+  if (!one) a.max_rows = 1;
+  a.max_len = pool ? std::min(c.context_len, bps * b2d::kKv4Page) : c.context_len;
+  a.dtype = B2D_BF16;
+  return a;
 }
 }  // namespace
 
@@ -513,11 +560,41 @@ b2d_status b2d_workspace_create(b2d_model* m, int max_batch, b2d_ws** out) {
   return B2D_OK;
 }
 
+b2d_status b2d_workspace_kv_bits(b2d_ws* ws, int bits) {
+  if (!ws || (bits != 16 && bits != 4)) return B2D_ERR_INVALID_ARG;
+  if (bits == 4 && !ws->q4) {
+    const b2d_config& c = ws->m->cfg;
+    B2D_CUDA(cudaSetDevice(ws->m->device), "cudaSetDevice");
+    // the most that the splits of any batch of rows, or of any prompt's chunk, need
+    uint64_t part = 16;
+    for (int n = 1; n <= ws->brows; ++n)
+      for (int one = 0; one < (n <= kPrefillRows ? 2 : 1); ++one) {
+        b2d::Kv4AttnArgs a = kv4_attn_args(ws, nullptr, nullptr, 0, 1, 1, n, one != 0, 0);
+        if (!b2d::kv4_attn_plan(a, ws->m->grid)) return B2D_ERR_UNSUPPORTED;
+        part = std::max(part, b2d::kv4_attn_scratch_most(a, ws->m->grid));
+      }
+    B2D_CUDA(cudaMalloc(&ws->kv4_part, part), "4-bit attention partials");
+    const cudaError_t e = cudaMalloc(&ws->q4, sizeof(__nv_bfloat16) * size_t(ws->brows) * c.n_heads * 64);
+    if (e != cudaSuccess) {
+      ws->q4 = nullptr;
+      cudaFree(ws->kv4_part);
+      ws->kv4_part = nullptr;
+      return cuda_fail(e, "4-bit attention queries");
+    }
+    ws->kv4_part_bytes = part;
+  }
+  ws->kv4 = bits == 4;
+  ++ws->tune_gen;  // cached step graphs belong to the other cache
+  return B2D_OK;
+}
+
 b2d_status b2d_workspace_destroy(b2d_ws* ws) {
   if (!ws) return B2D_OK;
   if (ws->m) cudaSetDevice(ws->m->device);
   for (auto& g : ws->graphs)
     if (g.exec) cudaGraphExecDestroy(g.exec);
+  cudaFree(ws->q4);
+  cudaFree(ws->kv4_part);
   cudaFree(ws->sample_scratch);
   cudaFreeHost(ws->tok_host);  // (tok_dev is its device alias)
   if (ws->cap_stream) cudaStreamDestroy(ws->cap_stream);
@@ -903,7 +980,8 @@ b2d_status run_rows(b2d_model* m, b2d_ws* ws, const int32_t* tok, const int32_t*
   // when the pool's rows of 64 bf16 are addressable with 32-bit coordinates.
   CUtensorMap kvmap{};
   const uint64_t pool_rows = uint64_t(c.n_layers) * uint64_t(num_blocks) * 2 * uint64_t(c.n_kv_heads) * b2d::kPageTokens;
-  const bool att_tma = table != nullptr && pool_rows <= 0x7fffffffull;
+  const bool kv4 = ws->kv4 && table != nullptr;  // (a contiguous cache is bf16 always)
+  const bool att_tma = !kv4 && table != nullptr && pool_rows <= 0x7fffffffull;
   if (att_tma) {
     if (ws->kvmap_pool != cache || ws->kvmap_nblk != num_blocks) {
       if (!b2d::make_kmajor_map(&ws->kvmap, cache, 64, pool_rows, b2d::kPageTokens)) return B2D_ERR_CUDA;
@@ -947,6 +1025,30 @@ b2d_status run_rows(b2d_model* m, b2d_ws* ws, const int32_t* tok, const int32_t*
                                                       : b2d::paged_attn_mma_kernel<2, true>;
   auto* att_k4 = att_tma ? b2d::paged_attn_mma_kernel<4, true> : b2d::paged_attn_mma_kernel<4, false>;
   const int att_smem2 = b2d::pa_smem_bytes(2, att_tma, att_stages);
+  // 4-bit pool: the rows are turned, quantised and appended, then attend; a
+  // prompt's rows (one table row for all) as the chunk of one sequence.
+  b2d::Kv4AppendArgs ka{};
+  b2d::Kv4AttnArgs kt{};
+  if (kv4) {
+    kt = kv4_attn_args(ws, pos, table, pa.table_ld, bps, num_blocks, batch, pa.table_ld == 0 && batch > 1, 0, cache);
+    if (!b2d::kv4_attn_plan(kt, m->grid) || b2d::kv4_attn_scratch(kt) > ws->kv4_part_bytes) return B2D_ERR_UNSUPPORTED;
+    ka.q = ws->qkv;
+    ka.k = ws->qkv + c.n_heads * 64;
+    ka.v = ws->qkv + (c.n_heads + c.n_kv_heads) * 64;
+    ka.q_out = ws->q4;
+    ka.q_row = ka.k_row = ka.v_row = Q;
+    ka.qo_row = D;
+    ka.q_head = ka.k_head = ka.v_head = ka.qo_head = 64;
+    ka.pos = pos;
+    ka.cos = pa.rcos;
+    ka.sin = pa.rsin;
+    ka.n_rows = batch;
+    ka.n_heads = c.n_heads;
+    ka.rotary = 64;
+    ka.max_pos = c.context_len;
+    ka.dtype = B2D_F32;
+    ka.q_out_dtype = B2D_BF16;
+  }
   // RMSNorm of the residual stream, folded: each residual projection writes
   // X = bf16(h * g_next) and per-tile sums of squares; the next projection
   // (qkv, gate/up, logits) scales its result columns by rsqrt(mean + eps).
@@ -958,16 +1060,22 @@ b2d_status run_rows(b2d_model* m, b2d_ws* ws, const int32_t* tok, const int32_t*
     pa.layer = l;
     pa.trace = ws->att_trace ? ws->att_trace + size_t(l) * kAttTraceUnits * 8 : nullptr;
     pa.trace_units = kAttTraceUnits;
-    if (prefill)  // every row's K/V in the cache before any row attends
+    if (kv4) {
+      kt.c = ka.c = kv4_cache(ws, cache, table, pa.table_ld, bps, num_blocks, batch, l);
+      B2D_CUDA(b2d::kv4_append(ka, st, pdl), "kv append");
+      B2D_CUDA(b2d::kv4_attention(kt, st, pdl), "attention");
+    } else if (prefill) {  // every row's K/V in the cache before any row attends
       B2D_CUDA(launch_k(b2d::kv_append_kernel, dim3(batch, c.n_kv_heads), dim3(32), st, pdl, pa), "kv append");
-    if (att_w == 2)
+    }
+    if (kv4) {
+    } else if (att_w == 2)
       B2D_CUDA(launch_k_smem(att_k2, dim3((att_units + 1) / 2), dim3(64), att_smem2, st, pdl, kvmap, pa, batch),
                "attention");
     else
       B2D_CUDA(launch_k_smem(att_k4, dim3((att_units + 3) / 4), dim3(128), b2d::pa_smem_bytes(4, att_tma), st, pdl,
                              kvmap, pa, batch),
                "attention");
-    launches_other += prefill ? 2 : 1;
+    launches_other += kv4 ? (kt.splits > 1 ? 3 : 2) : prefill ? 2 : 1;
     g.M = D; g.K = D; g.y = ws->Hm; g.resid = ws->H; g.ldy = D;
     g.ss_in = nullptr; g.xg_out = ws->X; g.xg_gain = ln2 + size_t(l) * D; g.ss_out = ws->ss;
     B2D_CUDA(gemm(m->wmaps[4 * l + 1], ws->amap, b2d::EPI_RESID_F32, p_o), "o");

@@ -106,6 +106,26 @@ cudaError_t kv4_read(const Kv4ReadArgs& a, cudaStream_t st) {
   return launch(kv4_read_kernel<__nv_bfloat16>, grid, block, 0, st, false, a);
 }
 
+namespace {
+int64_t plan_pages(const Kv4AttnArgs& a) { return std::max(1, (a.max_len + kKv4Page - 1) / kKv4Page); }
+int64_t plan_units(const Kv4AttnArgs& a) { return static_cast<int64_t>(a.n_seqs) * a.c.n_kv * a.tiles; }
+// Splits: at least 32 pages each (8 a warp).  One sequence's splits are alike:
+// one wave of CTAs, four to an SM (131071 positions, 8 kv heads of 128: 47 us,
+// and 55 us with splits for four waves).  Several sequences differ in length:
+// four waves even that out (32 of 1001 to 16384: 93 us, and 110 us with one).
+// Prompts: only where the tiles leave CTA slots empty, 64 pages each at least
+// (the join reads and writes every column's share: 274 us became 364).
+int64_t plan_splits(const Kv4AttnArgs& a, int sms) {
+  const bool prompt = a.tile_cols == kKv4PromptCols;
+  const int64_t ctas = int64_t(sms) * (prompt ? 2 : a.n_seqs == 1 ? 4 : 16), least = prompt ? 64 : 32;
+  return std::max<int64_t>(
+      1, std::min<int64_t>(ctas / std::max<int64_t>(1, plan_units(a)), (plan_pages(a) + least - 1) / least));
+}
+uint64_t scratch_of(const Kv4AttnArgs& a, int64_t splits) {
+  return splits <= 1 ? 0 : uint64_t(plan_units(a)) * splits * a.tile_cols * (a.c.d + 4) * sizeof(float);
+}
+}  // namespace
+
 bool kv4_attn_plan(Kv4AttnArgs& a, int sms) {
   a.group = a.n_heads / a.c.n_kv;
   a.group_inv = ((uint64_t(1) << 32) + a.group - 1) / a.group;
@@ -116,28 +136,15 @@ bool kv4_attn_plan(Kv4AttnArgs& a, int sms) {
   // 40 with tiles of 16; at 64 dims 24 and 17; 32 rows on 8000: 27 and 34).
   a.tile_cols = cols <= 8 ? 8 : cols <= 64 ? 16 : kKv4PromptCols;
   a.tiles = static_cast<int>((cols + a.tile_cols - 1) / a.tile_cols);
-  const int pages = std::max(1, (a.max_len + kKv4Page - 1) / kKv4Page);
-  const int64_t units = static_cast<int64_t>(a.n_seqs) * a.c.n_kv * a.tiles;
-  // Splits: at least 32 pages each (8 a warp).  One sequence's splits are alike:
-  // one wave of CTAs, four to an SM (131071 positions, 8 kv heads of 128: 45 us,
-  // and 55 us with splits for four waves).  Several sequences differ in length:
-  // four waves even that out (32 of 1001 to 16384: 93 us, and 110 us with one).
-  // Prompts: only where the tiles leave CTA slots empty, 64 pages each at least
-  // (the join reads and writes every column's share: 274 us became 364).
-  const bool prompt = a.tile_cols == kKv4PromptCols;
-  const int64_t ctas = int64_t(sms) * (prompt ? 2 : a.n_seqs == 1 ? 4 : 16), least = prompt ? 64 : 32;
-  const int64_t splits =
-      std::max<int64_t>(1, std::min<int64_t>(ctas / std::max<int64_t>(1, units), (pages + least - 1) / least));
+  const int64_t pages = plan_pages(a), splits = plan_splits(a, sms);
   a.split_pages = static_cast<int>((pages + splits - 1) / splits);
-  a.splits = (pages + a.split_pages - 1) / a.split_pages;
+  a.splits = static_cast<int>((pages + a.split_pages - 1) / a.split_pages);
   // the grid's y and z
   return a.c.n_kv <= 65535 && int64_t(a.tiles) * a.splits <= 65535 && (a.splits == 1 || cols <= 65535);
 }
 
-uint64_t kv4_attn_scratch(const Kv4AttnArgs& a) {
-  if (a.splits <= 1) return 0;
-  return uint64_t(a.n_seqs) * a.c.n_kv * a.tiles * a.splits * a.tile_cols * (a.c.d + 4) * sizeof(float);
-}
+uint64_t kv4_attn_scratch(const Kv4AttnArgs& a) { return scratch_of(a, a.splits); }
+uint64_t kv4_attn_scratch_most(const Kv4AttnArgs& a, int sms) { return scratch_of(a, plan_splits(a, sms)); }
 
 cudaError_t kv4_attention(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
   if (a.n_rows == 0 || a.n_seqs == 0) return cudaSuccess;

@@ -643,6 +643,7 @@ __device__ __forceinline__ bool kv4_tile(const Kv4AttnArgs& a, int z, Kv4Tile& t
   t.len = __ldg(a.lens + t.seq) + a.len_add;
   t.r0 = t.seq;
   t.rows = 1;
+  if (a.rows_of_one > 0) t.rows = a.rows_of_one;
   if (a.q_start != nullptr) {
     t.r0 = __ldg(a.q_start + t.seq);
     t.rows = __ldg(a.q_start + t.seq + 1) - t.r0;
@@ -651,8 +652,8 @@ __device__ __forceinline__ bool kv4_tile(const Kv4AttnArgs& a, int z, Kv4Tile& t
       if (threadIdx.x == 0) kv4_error(a.c.status, kKv4BadPos);
       return false;
     }
-    if (t.tile * a.tile_cols >= t.cols(a)) return false;
   }
+  if (t.tile * a.tile_cols >= t.cols(a)) return false;
   if (t.len > a.max_len) {
     if (threadIdx.x == 0) kv4_error(a.c.status, kKv4BadPos);
     t.len = 0;

@@ -50,7 +50,8 @@ struct Kv4AttnArgs {
   void* out;
   int64_t q_row, q_head, o_row, o_head;
   const int32_t* lens;     // [n_seqs]; len_add is added to each
-  const int32_t* q_start;  // [n_seqs + 1], or null: sequence i has the one row i
+  const int32_t* q_start;  // [n_seqs + 1], or null: sequence i has the one row i ..
+  int rows_of_one;         // .. or, when > 0, the one sequence has rows 0 .. rows_of_one - 1
   float* part;             // partials of split sequences (kv4_attn_scratch bytes)
   float scale_log2;        // softmax scale * log2(e)
   int n_rows, n_heads, n_seqs, max_rows, max_len, dtype;
@@ -68,6 +69,8 @@ cudaError_t kv4_read(const Kv4ReadArgs& a, cudaStream_t st);
 // a.part it needs.
 bool kv4_attn_plan(Kv4AttnArgs& a, int sms);
 uint64_t kv4_attn_scratch(const Kv4AttnArgs& a);
+// (planned) The most that it needs at this or a smaller max_len.
+uint64_t kv4_attn_scratch_most(const Kv4AttnArgs& a, int sms);
 cudaError_t kv4_attention(const Kv4AttnArgs& a, cudaStream_t st, bool pdl);
 
 }  // namespace b2d

@@ -22,6 +22,7 @@ import torch
 
 from . import _lib
 from .config import ModelConfig
+from .kv4 import page_bytes
 from .packing import kv_elems, new_kv_cache
 
 PAGE_TOKENS = 16  # positions per KV block of the paged pool
@@ -40,7 +41,12 @@ def _stream_ptr(stream) -> ctypes.c_void_p:
 class DecodeEngine:
     """A packed model bound to the C ABI plus one workspace."""
 
-    def __init__(self, w: dict, max_batch: int = 1):
+    def __init__(self, w: dict, max_batch: int = 1, kv_bits: int = 16):
+        """``kv_bits``: what the paged pools hold, 16 (bf16) or 4 (see ``kv4``:
+        3.6 times the positions in the same memory); the contiguous cache of
+        ``new_kv`` is bf16 either way."""
+        if kv_bits not in (16, 4):
+            raise ValueError("kv_bits must be 16 or 4")
         self.lib = _lib.load()
         self.w = w
         self.cfg: ModelConfig = w["config"]
@@ -58,11 +64,14 @@ class DecodeEngine:
         try:
             _lib.check(self.lib.b2d_workspace_create(self.model, max_batch, ctypes.byref(ws)),
                        "b2d_workspace_create")
+            if kv_bits != 16:
+                _lib.check(self.lib.b2d_workspace_kv_bits(ws, kv_bits), "b2d_workspace_kv_bits")
         except Exception:
+            self.lib.b2d_workspace_destroy(ws)
             self.lib.b2d_model_destroy(self.model)
             raise
         self.ws = ws
-        self.max_batch = max_batch
+        self.max_batch, self.kv_bits = max_batch, kv_bits
         self.grid = self.lib.b2d_model_grid(self.model)
         dev = self.device
         self.tok = torch.zeros(max_batch, dtype=torch.int32, device=dev)
@@ -154,13 +163,23 @@ class DecodeEngine:
 
     def new_kv_pool(self, num_blocks: int) -> torch.Tensor:
         """Zeroed paged KV pool: bf16 [n_layers, num_blocks, 2 (K|V), kv_heads,
-        16, d_head]; block i of a sequence holds its positions 16i..16i+15."""
+        16, d_head]; block i of a sequence holds its positions 16i..16i+15.
+        With ``kv_bits`` 4: uint8 [n_layers, num_blocks, kv_heads, 18 d_head]
+        (each layer's part is a ``kv4`` pool)."""
         c = self.cfg
+        if self.kv_bits == 4:
+            return torch.zeros(c.n_layers, num_blocks, c.n_kv_heads, page_bytes(c.d_head), dtype=torch.uint8,
+                               device=self.device)
         return torch.zeros(c.n_layers, num_blocks, 2, c.n_kv_heads, PAGE_TOKENS, c.d_head,
                            dtype=torch.bfloat16, device=self.device)
 
     def _check_pool(self, pool: torch.Tensor) -> None:
         c = self.cfg
+        if self.kv_bits == 4:
+            if (pool.dtype != torch.uint8 or pool.device != self.device or not pool.is_contiguous() or pool.dim() != 4
+                    or tuple(pool.shape[i] for i in (0, 2, 3)) != (c.n_layers, c.n_kv_heads, page_bytes(c.d_head))):
+                raise ValueError("pool must be a 4-bit paged KV pool of this model (see new_kv_pool)")
+            return
         if (pool.dtype != torch.bfloat16 or pool.device != self.device or not pool.is_contiguous() or pool.dim() != 6
                 or tuple(pool.shape[i] for i in (0, 2, 3, 4, 5)) != (c.n_layers, 2, c.n_kv_heads, PAGE_TOKENS,
                                                                      c.d_head)):

@@ -84,6 +84,10 @@ class Request:
     top_p: float = 1.0
     rep_penalty: float = 1.0
     seed: int | None = None
+    presence: float = 0.0
+    frequency: float = 0.0
+    logit_bias: dict | None = None
+    allowed: object = None   # token ids, or a function of the tokens generated that gives them
     out: list = dataclasses.field(default_factory=list)
     blocks: list = dataclasses.field(default_factory=list)
     slot: int = -1
@@ -94,7 +98,11 @@ class Request:
 
     @property
     def greedy(self) -> bool:
-        return self.temperature == 0.0 and self.rep_penalty == 1.0
+        return self.temperature == 0.0 and self.rep_penalty == 1.0 and not self.rules
+
+    @property
+    def rules(self) -> bool:
+        return bool(self.presence or self.frequency or self.logit_bias or self.allowed is not None)
 
     def next_pos(self) -> int:
         """Position of the token fed at this request's next decode row."""
@@ -194,7 +202,13 @@ class ContinuousBatcher:
 
     # ---- requests --------------------------------------------------------
     def submit(self, prompt, max_tokens: int, temperature: float = 0.0, top_p: float = 1.0,
-               rep_penalty: float = 1.0, seed: int | None = None) -> int:
+               rep_penalty: float = 1.0, seed: int | None = None, presence: float = 0.0, frequency: float = 0.0,
+               logit_bias: dict | None = None, allowed=None) -> int:
+        """Queues a request; returns its id.  ``presence`` and ``frequency`` are
+        subtracted from the logits of tokens it has generated, once and times
+        their count; ``logit_bias`` {token: value} is added; ``allowed`` are the
+        only token ids it may draw, or a function of the list of its generated
+        tokens that gives them (none: the request ends)."""
         prompt = np.asarray(prompt, dtype=np.int32).reshape(-1)
         if prompt.size == 0:
             raise ValueError("empty prompt")
@@ -209,13 +223,27 @@ class ContinuousBatcher:
             raise ValueError("bad sampling parameters")
         if max_tokens > self._hist_cap:
             raise ValueError("max_tokens exceeds the sampler history capacity")
+        bias = {int(t): float(v) for t, v in (logit_bias or {}).items()}
+        if any(not 0 <= t < self.vocab for t in bias) or not all(np.isfinite([presence, frequency, *bias.values()])):
+            raise ValueError("penalties and biases must be finite numbers, biases of tokens in the vocabulary")
+        if allowed is not None and not callable(allowed):
+            allowed = self._allowed_ids(allowed)
+            if not allowed.size:
+                raise ValueError("no token allowed")
         rid = self._next_rid
         self._next_rid += 1
-        r = Request(rid, prompt, int(max_tokens), float(temperature), float(top_p), float(rep_penalty), seed)
+        r = Request(rid, prompt, int(max_tokens), float(temperature), float(top_p), float(rep_penalty), seed,
+                    float(presence), float(frequency), bias or None, allowed)
         if not r.greedy:
             r.rng = np.random.RandomState(seed)
         self.waiting.append(r)
         return rid
+
+    def _allowed_ids(self, ids) -> np.ndarray:
+        ids = np.asarray(list(ids) if not isinstance(ids, np.ndarray) else ids, dtype=np.int64).reshape(-1)
+        if ids.size and (ids.min() < 0 or ids.max() >= self.vocab):
+            raise ValueError("allowed token out of range")
+        return ids
 
     @property
     def running(self) -> list[Request]:
@@ -433,11 +461,17 @@ class ContinuousBatcher:
     def _emit(self, rows, toks, events) -> None:
         self._tok_dirty = True
         for i, r in rows:
-            t = int(toks[i])
-            r.out.append(t)
-            events.append((r.rid, t))
-            self.stats["tokens"] += 1
-            self._maybe_finish(r)
+            self._take(r, int(toks[i]), events)
+
+    def _take(self, r: Request, t: int, events) -> None:
+        """The request's next token (negative: it allows none, and ends)."""
+        if t < 0:
+            self._finish(r)
+            return
+        r.out.append(t)
+        events.append((r.rid, t))
+        self.stats["tokens"] += 1
+        self._maybe_finish(r)
 
     def _admit(self, budget):
         """Admit waiting requests in order while a slot and the pages for their
@@ -526,10 +560,7 @@ class ContinuousBatcher:
                 toks = (self._sample_rows(logits, reqs, self._dp_next) if sampled
                         else self._fetch(self._dp_next, n_out))
                 for q, t in zip(reqs, toks):
-                    q.out.append(int(t))
-                    events.append((q.rid, int(t)))
-                    self.stats["tokens"] += 1
-                    self._maybe_finish(q)
+                    self._take(q, int(t), events)
             elif self._cuda:  # the pinned staging is rewritten by the next chunk
                 torch.cuda.current_stream(self.eng.device).synchronize()
             body.clear()
@@ -579,6 +610,9 @@ class ContinuousBatcher:
     def _maybe_finish(self, r: Request) -> None:
         if len(r.out) < r.max_tokens and (self.eos_id is None or r.out[-1] != self.eos_id):
             return
+        self._finish(r)
+
+    def _finish(self, r: Request) -> None:
         self.pages.free(r.blocks)
         r.blocks = []
         self.slots[r.slot] = None
@@ -612,6 +646,9 @@ class ContinuousBatcher:
         smp = self._sampler
         batch = len(rows)
         out = np.zeros(batch, np.int32)
+        ended = self._apply_rules(logits, rows)
+        rows = [None if i in ended else r for i, r in enumerate(rows)]
+        out[list(ended)] = -1
         groups: dict = {}
         for i, r in enumerate(rows):
             if r is not None and not r.greedy:
@@ -646,3 +683,45 @@ class ContinuousBatcher:
                 torch.index_select(logits, 0, self._d_idx[:m], out=lg)
             out[idx] = smp.sample(lg, temp, top_p, rp, m).cpu().numpy()[:m]
         return out
+
+    def _apply_rules(self, logits: torch.Tensor, rows) -> set:
+        """The rules of the requests ``rows`` on their rows of ``logits``, in
+        place, in one ``adjust_logits`` call; returns the rows that allow no token."""
+        ended = set()
+        if not any(r is not None and r.rules for r in rows):
+            return ended
+        from .generate import adjust_logits
+        n, words = len(rows), (self.vocab + 31) // 32
+        n_bias = max((len(r.logit_bias) for r in rows if r is not None and r.logit_bias), default=0)
+        masked = any(r is not None and r.allowed is not None for r in rows)
+        hist_cap = max([len(r.out) for r in rows if r is not None and r.rules] + [1])
+        hist, ints = np.zeros((n, hist_cap), np.int32), np.zeros((2, n), np.int32)  # lengths of history, biases
+        penalty = np.zeros((2, n), np.float32)  # presence, frequency
+        bias_ids, bias = np.zeros((n, n_bias), np.int32), np.zeros((n, n_bias), np.float32)
+        allow = np.full((n, 32 * words), 1, np.uint8) if masked else None
+        for i, r in enumerate(rows):
+            if r is None or not r.rules:
+                continue
+            hist[i, :len(r.out)], ints[0, i] = r.out, len(r.out)
+            penalty[:, i] = r.presence, r.frequency
+            if r.logit_bias:
+                k = ints[1, i] = len(r.logit_bias)
+                bias_ids[i, :k], bias[i, :k] = list(r.logit_bias), list(r.logit_bias.values())
+            if r.allowed is not None:
+                ids = self._allowed_ids(r.allowed(list(r.out))) if callable(r.allowed) else r.allowed
+                if not ids.size:
+                    ended.add(i)
+                allow[i] = 0
+                allow[i, ids] = 1
+
+        def put(a):
+            return torch.from_numpy(np.ascontiguousarray(a)).to(self.eng.device)
+
+        lens = put(ints)
+        kw = dict(history=put(hist), hist_len=lens[0], presence=put(penalty[0]), frequency=put(penalty[1]))
+        if n_bias:
+            kw.update(bias_ids=put(bias_ids), bias_values=put(bias), bias_len=lens[1])
+        if masked:
+            kw["allowed"] = put(np.packbits(allow, axis=1, bitorder="little").view(np.int32))
+        adjust_logits(logits[:n], out=logits[:n], **kw)
+        return ended
