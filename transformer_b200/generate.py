@@ -37,7 +37,7 @@ import torch
 
 from . import _lib
 from .config import ModelConfig
-from .kv4 import _empty, _stream_on
+from .kv4 import _empty_like, _stream_on
 from .multi_sm_decode import DecodeEngine, _ptr, _stream_ptr
 from .packing import prepare_decode_weights_nlayer
 
@@ -96,15 +96,18 @@ def adjust_logits(logits, *, out=None, history=None, hist_len=None, prompt_len=N
       word v // 32; tokens whose bit is 0 become -infinity.
 
     In this order; ids outside the vocabulary count for nothing."""
-    dev = logits.device
-    if logits.dtype != torch.float32 or logits.dim() != 2 or dev.type != "cuda":
+    dev = logits.get_device()
+    if logits.dtype is not torch.float32 or logits.dim() != 2 or dev < 0:
         raise ValueError("logits must be float32 [batch, vocab] on a GPU")
-    batch, vocab = logits.shape
+    batch, vocab = shape = logits.shape
     if out is None:
-        out = _empty(logits.shape, torch.float32, dev, stream)
-    ld, out_ld = logits.stride(0) if batch > 1 else vocab, out.stride(0) if batch > 1 else vocab
-    if vocab < 1 or out.dtype != torch.float32 or out.shape != logits.shape or out.device != dev or (
-            vocab > 1 and (logits.stride(1) != 1 or out.stride(1) != 1)) or min(ld, out_ld) < vocab:
+        out = _empty_like(logits, stream)
+    ld, one = logits.stride()
+    out_ld, out_one = out.stride() if out.dim() == 2 else (0, 0)
+    if batch <= 1:
+        ld = out_ld = vocab
+    if vocab < 1 or out.dtype is not torch.float32 or out.shape != shape or out.get_device() != dev or (
+            vocab > 1 and (one != 1 or out_one != 1)) or ld < vocab or out_ld < vocab:
         raise ValueError("logits and out must be float32 [batch, vocab] on one GPU, their rows contiguous and apart")
     if (history is None) != (hist_len is None):
         raise ValueError("history and hist_len go together")
@@ -112,31 +115,30 @@ def adjust_logits(logits, *, out=None, history=None, hist_len=None, prompt_len=N
         raise ValueError("penalties need the history")
     if (bias_ids is None) != (bias_values is None) or (bias_ids is None) != (bias_len is None):
         raise ValueError("bias_ids, bias_values and bias_len go together")
-    one = (batch,)
+    row = (batch,)
     cap = history.shape[-1] if history is not None else 0
     n_bias = bias_ids.shape[-1] if bias_ids is not None else 0
     words = allowed.shape[-1] if allowed is not None else 0
     if allowed is not None and 32 * words < vocab:
         raise ValueError(f"allowed must have {(vocab + 31) // 32} words a row")
-    ptrs = []
-    for t, name, dtype, shape in (
-            (history, "history", torch.int32, (batch, cap)), (hist_len, "hist_len", torch.int32, one),
-            (prompt_len, "prompt_len", torch.int32, one), (rep_penalty, "rep_penalty", torch.float32, one),
-            (presence, "presence", torch.float32, one), (frequency, "frequency", torch.float32, one),
-            (bias_ids, "bias_ids", torch.int32, (batch, n_bias)),
-            (bias_values, "bias_values", torch.float32, (batch, n_bias)), (bias_len, "bias_len", torch.int32, one),
-            (allowed, "allowed", torch.int32, (batch, words))):
+
+    def take(t, name, dtype, shape):
         if t is None:
-            ptrs.append(None)
-        elif t.dtype != dtype or t.shape != shape or t.device != dev or not t.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on {dev}")
-        else:
-            ptrs.append(t.data_ptr())
-    if not batch:
-        return out
-    r = _lib.LogitsRules(logits.data_ptr(), out.data_ptr(), ld, out_ld, *ptrs, words, batch, vocab, cap, n_bias,
-                         dev.index)
-    _lib.check(_lib.load().b2d_adjust_logits(ctypes.byref(r), _stream_on(stream, dev)), "b2d_adjust_logits")
+            return None
+        if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous {dtype} tensor of shape {list(shape)} on the logits' device")
+        return t.data_ptr()
+
+    i32, f32 = torch.int32, torch.float32
+    r = _lib.LogitsRules(
+        logits.data_ptr(), out.data_ptr(), ld, out_ld, take(history, "history", i32, (batch, cap)),
+        take(hist_len, "hist_len", i32, row), take(prompt_len, "prompt_len", i32, row),
+        take(rep_penalty, "rep_penalty", f32, row), take(presence, "presence", f32, row),
+        take(frequency, "frequency", f32, row), take(bias_ids, "bias_ids", i32, (batch, n_bias)),
+        take(bias_values, "bias_values", f32, (batch, n_bias)), take(bias_len, "bias_len", i32, row),
+        take(allowed, "allowed", i32, (batch, words)), words, batch, vocab, cap, n_bias, dev)
+    if batch:
+        _lib.check(_lib.load().b2d_adjust_logits(ctypes.byref(r), _stream_on(stream, dev)), "b2d_adjust_logits")
     return out
 
 

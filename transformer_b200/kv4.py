@@ -17,6 +17,7 @@ first) and skip the access; ``check_status`` raises for it.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -26,17 +27,17 @@ PAGE_TOKENS = 16  # positions per block
 _TYPES = {torch.float32: _lib.B2D_F32, torch.bfloat16: _lib.B2D_BF16, torch.float16: _lib.B2D_F16}
 
 
-def _stream_on(stream, device) -> int:
-    """The stream's handle, by default the current one of ``device``."""
-    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(device.index)
+def _stream_on(stream, index) -> int:
+    """The stream's handle, by default the current one of the device `index`."""
+    return stream.cuda_stream if stream is not None else torch._C._cuda_getCurrentRawStream(index)
 
 
-def _empty(shape, dtype, device, stream) -> torch.Tensor:
+def _empty_like(t, stream, dtype=None) -> torch.Tensor:
     """A tensor from the stream's own memory (as torch's allocator keeps it)."""
     if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty_like(t, dtype=dtype)
     with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
+        return torch.empty_like(t, dtype=dtype)
 
 
 def page_bytes(d_head: int) -> int:
@@ -58,45 +59,57 @@ def check_status(status: torch.Tensor) -> None:
         raise _lib.B2DError(_lib.B2D_ERR_DEVICE_INPUT, "device status", f"word 0x{word & 0xffffffff:x}")
 
 
-def _ints(t, name, device, n):
-    if t.dtype != torch.int32 or t.shape != (n,) or t.device != device or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} items on {device}")
+def _ints(t, name, index, n):
+    if t.dtype is not torch.int32 or t.shape != (n,) or t.get_device() != index or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} items on the pool's device")
     return t.data_ptr()
 
 
-def _cache(pool, table, status, n_kv, d) -> _lib.Kv4Cache:
-    dev = pool.device
-    if dev.type != "cuda":
+def _cache(pool, table, status):
+    """(the C cache, its device, blocks_per_seq, table rows, kv heads, dims)"""
+    index = pool.get_device()
+    if index < 0:
         raise ValueError("pool must be on a GPU")
-    blocks = pool.shape[0]
-    if pool.dtype != torch.uint8 or pool.shape != (blocks, n_kv, 18 * d) or blocks < 1 or not pool.is_contiguous():
-        raise ValueError(f"pool must be contiguous uint8 [num_blocks, {n_kv}, {18 * d}] (see new_kv4_pool)")
-    if table.dtype != torch.int32 or table.dim() != 2 or table.device != dev or not table.is_contiguous() or (
-            table.numel() < 1):
+    if pool.dtype is not torch.uint8 or pool.dim() != 3 or not pool.is_contiguous():
+        raise ValueError("pool must be contiguous uint8 [num_blocks, n_kv, 18 * d_head] (see new_kv4_pool)")
+    blocks, n_kv, size = pool.shape
+    if size not in (1152, 2304) or n_kv < 1 or blocks < 1:
+        raise ValueError("pool must hold heads of 64 or 128 dims: uint8 [num_blocks, n_kv, 18 * d_head]")
+    if table.dtype is not torch.int32 or table.dim() != 2 or table.get_device() != index or not table.is_contiguous():
         raise ValueError("table must be a contiguous int32 [n_seqs, blocks_per_seq] tensor on the pool's device")
-    if status is not None and (status.dtype != torch.int32 or status.device != dev or status.numel() != 1):
-        raise ValueError("status must be an int32 tensor of one item on the pool's device")
     rows, bps = table.shape
-    return _lib.Kv4Cache(pool.data_ptr(), table.data_ptr(), None if status is None else status.data_ptr(), n_kv, d,
-                         blocks, bps, rows, dev.index)
+    if rows < 1 or bps < 1:
+        raise ValueError("table must name a block")
+    if status is not None and (status.dtype is not torch.int32 or status.get_device() != index or status.numel() != 1):
+        raise ValueError("status must be an int32 tensor of one item on the pool's device")
+    d = size // 18
+    return (_lib.Kv4Cache(pool.data_ptr(), table.data_ptr(), None if status is None else status.data_ptr(), n_kv, d,
+                          blocks, bps, rows, index), index, bps, rows, n_kv, d)
 
 
-def _strides(t, name, device, shape, types):
+def _strides(t, name, index, shape, types):
     """(address, row stride, head stride) of a [rows, heads, d] tensor with
     contiguous dims and any row and head strides."""
-    if t.shape != shape or t.dtype not in types or t.device != device:
-        raise ValueError(f"{name} must be a {list(shape)} tensor on {device}, of " + " or ".join(map(str, types)))
+    if t.shape != shape or t.dtype not in types or t.get_device() != index:
+        raise ValueError(f"{name} must be a {list(shape)} tensor on the pool's device, of "
+                         + " or ".join(map(str, types)))
     row, head, one = t.stride()
     if one != 1:
         raise ValueError(f"{name} must have contiguous dims")
     return t.data_ptr(), row, head
 
 
-def _pool_heads(pool):
-    """(kv heads, dims) that a pool holds."""
-    if pool.dim() != 3 or pool.shape[2] % 18:
-        raise ValueError("pool must be uint8 [num_blocks, n_kv, 18 * d_head] (see new_kv4_pool)")
-    return pool.shape[1], pool.shape[2] // 18
+@functools.lru_cache(maxsize=4096)
+def _scratch_bytes(index, n_kv, d, heads, n_seqs, max_rows, max_len) -> int:
+    """Bytes of scratch that a call of these sizes needs (a function of them alone)."""
+    room = (max_len + PAGE_TOKENS - 1) // PAGE_TOKENS or 1
+    cache = _lib.Kv4Cache(16, 16, None, n_kv, d, 1, room, n_seqs, index)  # (addresses that the query does not read)
+    query = _lib.Kv4Query(16, 16, 0, 0, 0, 0, 16, 16, _lib.B2D_F16, max(max_rows, n_seqs), heads, n_seqs, max_rows,
+                          max_len, 1.0)
+    need = ctypes.c_uint64()
+    _lib.check(_lib.load().b2d_kv4_attention_scratch(ctypes.byref(cache), ctypes.byref(query), ctypes.byref(need)),
+               "b2d_kv4_attention_scratch")
+    return need.value
 
 
 def kv4_append(pool, k, v, pos, table, *, seq=None, q=None, q_out=None, cos=None, sin=None, interleaved=False,
@@ -111,13 +124,12 @@ def kv4_append(pool, k, v, pos, table, *, seq=None, q=None, q_out=None, cos=None
     rotation.  ``q`` [n, heads, d] is turned alike into ``q_out`` (default: a
     new tensor; may be ``q``; a float32 ``q`` also into bf16 or fp16), which is
     returned.  Two rows at one position: the cache gets dims of either."""
-    n_kv, d = _pool_heads(pool)
-    c = _cache(pool, table, status, n_kv, d)
-    dev, n = pool.device, pos.numel()
+    c, dev, _, table_rows, n_kv, d = _cache(pool, table, status)
+    n = pos.numel()
     shape = (n, n_kv, d)
     k_ptr, k_row, k_head = _strides(k, "k", dev, shape, _TYPES)
     v_ptr, v_row, v_head = _strides(v, "v", dev, shape, (k.dtype,))
-    if seq is None and n > table.shape[0]:
+    if seq is None and n > table_rows:
         raise ValueError("more rows than table rows need seq")
     heads = rotary = max_pos = q_row = q_head = o_row = o_head = 0
     q_ptr = o_ptr = None
@@ -128,11 +140,11 @@ def kv4_append(pool, k, v, pos, table, *, seq=None, q=None, q_out=None, cos=None
         if heads < 1:
             raise ValueError("q needs a head")
         if q_out is None:
-            q_out = _empty(q.shape, q.dtype, dev, stream)
-        o_ptr, o_row, o_head = _strides(q_out, "q_out", dev, q.shape,
-                                        _TYPES if q.dtype == torch.float32 else (q.dtype,))
+            q_out = _empty_like(q, stream)
+        o_ptr, o_row, o_head = _strides(q_out, "q_out", dev, (n, heads, d),
+                                        _TYPES if q.dtype is torch.float32 else (q.dtype,))
         o_type = _TYPES[q_out.dtype]
-        if o_ptr == q_ptr and n and (q_out.stride() != q.stride() or o_type != dtype):
+        if o_ptr == q_ptr and n and (o_row != q_row or o_head != q_head or o_type != dtype):
             raise ValueError("q_out must be q or apart from it")
     elif q_out is not None:
         raise ValueError("q_out without q")
@@ -142,9 +154,10 @@ def kv4_append(pool, k, v, pos, table, *, seq=None, q=None, q_out=None, cos=None
         max_pos, half = cos.shape if cos.dim() == 2 else (0, 0)
         rotary = 2 * half
         for t in (cos, sin):
-            if t.dtype != torch.float32 or t.shape != (max_pos, half) or t.device != dev or not t.is_contiguous() or (
-                    not 2 <= rotary <= d) or max_pos < 1:
-                raise ValueError(f"cos and sin must be contiguous float32 [max_pos, r / 2] on {dev}, 2 <= r <= {d}")
+            if t.dtype is not torch.float32 or t.shape != (max_pos, half) or t.get_device() != dev or (
+                    not t.is_contiguous()) or not 2 <= rotary <= d or max_pos < 1:
+                raise ValueError(f"cos and sin must be contiguous float32 [max_pos, r / 2] on the pool's device, "
+                                 f"2 <= r <= {d}")
     r = _lib.Kv4Rows(q_ptr, k_ptr, v_ptr, o_ptr, q_row, q_head, k_row, k_head, v_row, v_head, o_row, o_head,
                      _ints(pos, "pos", dev, n), None if seq is None else _ints(seq, "seq", dev, n),
                      None if cos is None else cos.data_ptr(), None if sin is None else sin.data_ptr(), dtype, o_type, n,
@@ -159,15 +172,19 @@ def kv4_read(pool, pos, table, *, seq=None, dtype=torch.bfloat16, status=None, s
     """The rows at positions ``pos`` of the sequences ``seq`` (as in
     ``kv4_append``) as values: ``(k, v)``, each [n, n_kv, d] of ``dtype``
     (float32, bf16 or fp16, all exact); zeros where ``pos`` is negative."""
-    n_kv, d = _pool_heads(pool)
-    c = _cache(pool, table, status, n_kv, d)
-    dev, n = pool.device, pos.numel()
+    c, dev, _, table_rows, n_kv, d = _cache(pool, table, status)
+    n = pos.numel()
     if dtype not in _TYPES:
         raise ValueError("dtype must be float32, bfloat16 or float16")
-    if seq is None and n > table.shape[0]:
+    if seq is None and n > table_rows:
         raise ValueError("more rows than table rows need seq")
     p, s = _ints(pos, "pos", dev, n), None if seq is None else _ints(seq, "seq", dev, n)
-    k, v = (_empty((n, n_kv, d), dtype, dev, stream) for _ in range(2))
+    if stream is None:
+        k = pool.new_empty((n, n_kv, d), dtype=dtype)
+    else:
+        with torch.cuda.stream(stream):
+            k = pool.new_empty((n, n_kv, d), dtype=dtype)
+    v = _empty_like(k, stream)
     if n:
         _lib.check(_lib.load().b2d_kv4_read(ctypes.byref(c), p, s, n, _TYPES[dtype], k.data_ptr(), v.data_ptr(),
                                             _stream_on(stream, dev)), "b2d_kv4_read")
@@ -189,19 +206,18 @@ def kv4_attention(q, pool, lens, table, *, q_start=None, max_rows=None, max_len=
     ``max_rows`` (default: n), and rows of no sequence stay as they are.
     ``max_len`` (default: what a table row holds) bounds ``lens``; a close
     bound splits long sequences better.  ``scale`` defaults to d ** -0.5."""
-    n_kv, d = _pool_heads(pool)
-    c = _cache(pool, table, status, n_kv, d)
-    dev = pool.device
+    c, dev, bps, table_rows, n_kv, d = _cache(pool, table, status)
     n, heads = q.shape[:2] if q.dim() == 3 else (0, 0)
-    q_ptr, q_row, q_head = _strides(q, "q", dev, (n, heads, d), _QUERY_TYPES)
+    shape = (n, heads, d)
+    q_ptr, q_row, q_head = _strides(q, "q", dev, shape, _QUERY_TYPES)
     if heads < 1 or heads % n_kv:
         raise ValueError(f"q must have a multiple of {n_kv} heads")
-    n_seqs, (rows, bps) = lens.numel(), table.shape
-    if n_seqs > rows:
+    n_seqs = lens.numel()
+    if n_seqs > table_rows:
         raise ValueError("more lengths than table rows")
     if out is None:
-        out = _empty(q.shape, q.dtype, dev, stream)
-    o_ptr, o_row, o_head = _strides(out, "out", dev, q.shape, (q.dtype,))
+        out = _empty_like(q, stream)
+    o_ptr, o_row, o_head = _strides(out, "out", dev, shape, (q.dtype,))
     room = min(bps * PAGE_TOKENS, 2 ** 31 - 1)
     max_len = room if max_len is None else int(max_len)
     if not 0 <= max_len <= room:
@@ -216,21 +232,22 @@ def kv4_attention(q, pool, lens, table, *, q_start=None, max_rows=None, max_len=
         max_rows = max(1, n) if max_rows is None else int(max_rows)
         if max_rows < 1:
             raise ValueError("max_rows must be at least 1")
+        max_rows = min(max_rows, max(1, n))
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < float("inf"):
         raise ValueError("scale must be positive")
     if not n or not n_seqs:
         return out
-    lib, stream_ptr = _lib.load(), _stream_on(stream, dev)
+    need, scratch_ptr = _scratch_bytes(dev, n_kv, d, heads, n_seqs, max_rows, max_len), None
+    if need:  # from the stream's own memory: calls on other streams, and other graphs, have theirs
+        if stream is None:
+            scratch = pool.new_empty(need)
+        else:
+            with torch.cuda.stream(stream):
+                scratch = pool.new_empty(need)
+        scratch_ptr = scratch.data_ptr()
     query = _lib.Kv4Query(q_ptr, o_ptr, q_row, q_head, o_row, o_head, lens_ptr, start_ptr, _TYPES[q.dtype], n, heads,
                           n_seqs, max_rows, max_len, scale)
-    need = ctypes.c_uint64()
-    _lib.check(lib.b2d_kv4_attention_scratch(ctypes.byref(c), ctypes.byref(query), ctypes.byref(need)),
-               "b2d_kv4_attention_scratch")
-    scratch = None
-    if need.value:  # from the stream's own memory: calls on other streams, and other graphs, have theirs
-        scratch = _empty(need.value, torch.uint8, dev, stream)
-    _lib.check(lib.b2d_kv4_attention(ctypes.byref(c), ctypes.byref(query),
-                                     None if scratch is None else scratch.data_ptr(), need.value, stream_ptr),
-               "b2d_kv4_attention")
+    _lib.check(_lib.load().b2d_kv4_attention(ctypes.byref(c), ctypes.byref(query), scratch_ptr, need,
+                                             _stream_on(stream, dev)), "b2d_kv4_attention")
     return out
