@@ -2,6 +2,7 @@
 // (b2d_kv4_* in include/b2d.h).
 #include <algorithm>
 #include <atomic>
+#include <climits>
 #include <cmath>
 #include <cstring>
 
@@ -53,22 +54,21 @@ cudaError_t join(const Kv4AttnArgs& a, cudaStream_t st) {
 }
 
 template <auto Kernel, int Threads, int Smem, class T, int NH>
-cudaError_t launch_tiles(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
+cudaError_t launch_tiles(const Kv4AttnArgs& a, dim3 grid, cudaStream_t st, bool pdl) {
   cudaError_t e = raise_smem<Kernel, Smem>();
-  if (e == cudaSuccess)
-    e = launch(Kernel,
-               dim3(static_cast<unsigned>(a.n_seqs), static_cast<unsigned>(a.c.n_kv),
-                    static_cast<unsigned>(a.tiles * a.splits)),
-               dim3(Threads), Smem, st, pdl, a);
+  if (e == cudaSuccess) e = launch(Kernel, grid, dim3(Threads), Smem, st, pdl, a);
   return e == cudaSuccess ? join<T, NH>(a, st) : e;
 }
 template <class T, int NH, int NB>
 cudaError_t attn_launch(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
-  return launch_tiles<kv4_attn_kernel<T, NH, NB>, 32 * kKv4Warps, kv4_attn_smem<NH, NB>(), T, NH>(a, st, pdl);
+  const dim3 grid(static_cast<unsigned>(a.n_seqs), static_cast<unsigned>(a.c.n_kv),
+                  static_cast<unsigned>(a.tiles * a.splits));
+  return launch_tiles<kv4_attn_kernel<T, NH, NB>, 32 * kKv4Warps, kv4_attn_smem<NH, NB>(), T, NH>(a, grid, st, pdl);
 }
 template <class T, int NH>
 cudaError_t prompt_launch(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
-  return launch_tiles<kv4_prompt_kernel<T, NH>, kKv4PromptThreads, kv4_prompt_smem<NH>(), T, NH>(a, st, pdl);
+  const dim3 grid(static_cast<unsigned>(a.n_seqs) * a.c.n_kv * a.tiles, static_cast<unsigned>(a.splits));
+  return launch_tiles<kv4_prompt_kernel<T, NH>, kKv4PromptThreads, kv4_prompt_smem<NH>(), T, NH>(a, grid, st, pdl);
 }
 
 template <class T, int NH>
@@ -139,8 +139,8 @@ bool kv4_attn_plan(Kv4AttnArgs& a, int sms) {
   const int64_t pages = plan_pages(a), splits = plan_splits(a, sms);
   a.split_pages = static_cast<int>((pages + splits - 1) / splits);
   a.splits = static_cast<int>((pages + a.split_pages - 1) / a.split_pages);
-  // the grid's y and z
-  return a.c.n_kv <= 65535 && int64_t(a.tiles) * a.splits <= 65535 && (a.splits == 1 || cols <= 65535);
+  // the grid's x, y and z
+  return plan_units(a) <= INT_MAX && a.c.n_kv <= 65535 && int64_t(a.tiles) * a.splits <= 65535 && (a.splits == 1 || cols <= 65535);
 }
 
 uint64_t kv4_attn_scratch(const Kv4AttnArgs& a) { return scratch_of(a, a.splits); }

@@ -619,8 +619,7 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   return y;
 }
 
-// Where a CTA's work lies.  Grid: x = sequence, y = kv head, z = tile of query
-// columns + tiles * split.
+// Where a CTA's work lies.
 struct Kv4Tile {
   int seq, g, tile, split;
   int r0, rows, len;
@@ -633,13 +632,14 @@ __device__ __forceinline__ int kv4_row(const Kv4AttnArgs& a, int col) {  // col 
 __device__ __forceinline__ int kv4_limit(const Kv4AttnArgs& a, const Kv4Tile& t, int c) {
   return t.rows == 1 ? t.len : min(t.len, max(0, t.len - t.rows + kv4_row(a, c) + 1));
 }
+// Tile of query columns and split of kv head g of sequence seq.
 // False when the tile has no columns.  Bad inputs (lengths past the table or
 // max_len, rows past n_rows or max_rows) leave rows or len 0 and set the status.
-__device__ __forceinline__ bool kv4_tile(const Kv4AttnArgs& a, int z, Kv4Tile& t) {
-  t.seq = blockIdx.x;
-  t.g = blockIdx.y;
-  t.split = a.tiles == 1 ? z : z / a.tiles;
-  t.tile = z - t.split * a.tiles;
+__device__ __forceinline__ bool kv4_tile(const Kv4AttnArgs& a, int seq, int g, int tile, int split, Kv4Tile& t) {
+  t.seq = seq;
+  t.g = g;
+  t.tile = tile;
+  t.split = split;
   t.len = __ldg(a.lens + t.seq) + a.len_add;
   t.r0 = t.seq;
   t.rows = 1;
@@ -735,7 +735,9 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
   pdl_wait();
   pdl_launch();
   Kv4Tile tl;
-  if (!kv4_tile(a, blockIdx.z, tl)) return;
+  // grid: x = sequence, y = kv head, z = tile + tiles * split
+  const int split = a.tiles == 1 ? blockIdx.z : blockIdx.z / a.tiles;
+  if (!kv4_tile(a, blockIdx.x, blockIdx.y, blockIdx.z - split * a.tiles, split, tl)) return;
   const int pages = kv4_tile_pages(a, tl);
   const int lo = tl.split * a.split_pages, hi = min(pages, lo + a.split_pages);
   if (lo >= hi && tl.split > 0) return;  // (the first split always answers)
@@ -1041,7 +1043,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ K
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c = blockIdx.z, tile = c / a.tile_cols;
   Kv4Tile tl;
-  if (!kv4_tile(a, tile, tl) || c >= tl.cols(a)) return;
+  if (!kv4_tile(a, blockIdx.x, blockIdx.y, tile, 0, tl) || c >= tl.cols(a)) return;
   const int n = max(1, (kv4_tile_pages(a, tl) + a.split_pages - 1) / a.split_pages);
   const float* src = kv4_part(a, tl.seq, tl.g, tile, 0, c - tile * a.tile_cols, D);
   const int64_t step = static_cast<int64_t>(a.tile_cols) * (D + 4);

@@ -38,6 +38,7 @@
 // the largest keep their 11 bits.
 #pragma once
 
+#include <climits>
 #include <type_traits>
 
 #include "kv4.cuh"
@@ -123,6 +124,23 @@ struct Kv4Frag {
   uint32_t scale[NH];
 };
 
+// The sequence that is rank-th from the longest (equal lengths in their order):
+// the longest tiles start first, so that short ones fill the end (the same case:
+// 274 us in the sequences' order).  Whole warp.  More than 32 sequences stay in
+// their order: with so many tiles the last ones are a small part.
+__device__ __forceinline__ int kv4_seq_of_rank(const Kv4AttnArgs& a, int rank) {
+  if (a.n_seqs > 32 || a.n_seqs == 1) return rank;
+  const int lane = threadIdx.x & 31;
+  const int len = lane < a.n_seqs ? __ldg(a.lens + lane) : INT_MIN;
+  int before = 0;
+  for (int i = 0; i < a.n_seqs; ++i) {
+    const int other = __shfl_sync(0xffffffffu, len, i);
+    before += other > len || (other == len && i < lane);
+  }
+  return __ffs(__ballot_sync(0xffffffffu, lane < a.n_seqs && before == rank)) - 1;
+}
+
+// Grid: x = (rank * kv heads + kv head) * tiles + tile from the last, y = split.
 template <class T, int NH>
 __global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const __grid_constant__ Kv4AttnArgs a) {
   constexpr int D = 64 * NH, PB = kv4_page_bytes(D), PAGES = kKv4PromptKeys / kKv4Page;
@@ -139,7 +157,9 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const 
   constexpr int K_BUF = NH * 64 * 128, V_BUF = D * 128;
   pdl_wait();
   Kv4Tile tl;
-  const bool work = kv4_tile(a, blockIdx.z, tl);
+  const unsigned unit = blockIdx.x / a.tiles, rank = unit / a.c.n_kv;
+  const bool work = kv4_tile(a, kv4_seq_of_rank(a, rank), unit - rank * a.c.n_kv,
+                             a.tiles - 1 - static_cast<int>(blockIdx.x - unit * a.tiles), blockIdx.y, tl);
   const int pages = work ? kv4_tile_pages(a, tl) : 0;
   const int lo = tl.split * a.split_pages, hi = min(pages, lo + a.split_pages);
   if (!work || (lo >= hi && tl.split > 0)) {  // (the first split always answers)
