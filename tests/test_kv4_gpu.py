@@ -311,6 +311,26 @@ def test_attention_several_rows(cuda, dtype, heads, n_kv, d, lens, rows):
     check_attention(cuda, rng, dtype, heads, n_kv, d, lens, rows, extra_rows=3)
 
 
+@pytest.mark.parametrize("dtype,heads,n_kv,d", [("bf16", 16, 4, 64), ("f16", 8, 2, 128), ("bf16", 4, 4, 128)])
+def test_attention_many_chunks(cuda, dtype, heads, n_kv, d):
+    """More tiles of columns than SMs, so that a CTA takes two groups of them,
+    the second one empty here and there: more sequences than are put in order of
+    their lengths, and few of equal and unequal lengths."""
+    rng = np.random.default_rng(heads + d)
+    rows = [int(rng.integers(0, 161)) for _ in range(44)]
+    check_attention(cuda, rng, dtype, heads, n_kv, d, [r + int(rng.integers(0, 60)) for r in rows], rows, extra_rows=2)
+    rows = [600, 33, 350, 0, 600]
+    check_attention(cuda, rng, dtype, heads, n_kv, d, [700, 90, 400, 90, 700], rows)
+
+
+@pytest.mark.parametrize("dtype,heads,n_kv,d", [("bf16", 4, 4, 64), ("f16", 8, 2, 128)])
+def test_attention_split_chunks(cuda, dtype, heads, n_kv, d):
+    """Few columns on many positions, split and joined; one sequence has fewer splits."""
+    rng = np.random.default_rng(heads)
+    check_attention(cuda, rng, dtype, heads, n_kv, d, [5003, 1100, 70], [70, 66, 70])
+    check_attention(cuda, rng, dtype, heads, n_kv, d, [4097], [150])
+
+
 def test_attention_large_scores_and_scales(cuda):
     rng = np.random.default_rng(5)
     check_attention(cuda, rng, "bf16", 4, 2, 64, [100, 333], scale=3.0)

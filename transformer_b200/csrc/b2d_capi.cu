@@ -565,14 +565,7 @@ b2d_status b2d_workspace_kv_bits(b2d_ws* ws, int bits) {
   if (bits == 4 && !ws->q4) {
     const b2d_config& c = ws->m->cfg;
     B2D_CUDA(cudaSetDevice(ws->m->device), "cudaSetDevice");
-    // the most that the splits of any batch of rows, or of any prompt's chunk, need
-    uint64_t part = 16;
-    for (int n = 1; n <= ws->brows; ++n)
-      for (int one = 0; one < (n <= kPrefillRows ? 2 : 1); ++one) {
-        b2d::Kv4AttnArgs a = kv4_attn_args(ws, nullptr, nullptr, 0, 1, 1, n, one != 0, 0);
-        if (!b2d::kv4_attn_plan(a, ws->m->grid)) return B2D_ERR_UNSUPPORTED;
-        part = std::max(part, b2d::kv4_attn_scratch_most(a, ws->m->grid));
-      }
+    const uint64_t part = b2d::kv4_attn_scratch_most(64, ws->m->grid);
     B2D_CUDA(cudaMalloc(&ws->kv4_part, part), "4-bit attention partials");
     const cudaError_t e = cudaMalloc(&ws->q4, sizeof(__nv_bfloat16) * size_t(ws->brows) * c.n_heads * 64);
     if (e != cudaSuccess) {

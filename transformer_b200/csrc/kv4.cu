@@ -49,7 +49,7 @@ cudaError_t join(const Kv4AttnArgs& a, cudaStream_t st) {
   if (a.splits == 1) return cudaSuccess;
   return launch(kv4_join_kernel<T, NH>,
                 dim3(static_cast<unsigned>(a.n_seqs), static_cast<unsigned>(a.c.n_kv),
-                     static_cast<unsigned>(a.max_rows * a.group)),
+                     static_cast<unsigned>((a.max_rows * a.group + 3) / 4)),
                 dim3(128), 0, st, true, a);
 }
 
@@ -65,15 +65,17 @@ cudaError_t attn_launch(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
                   static_cast<unsigned>(a.tiles * a.splits));
   return launch_tiles<kv4_attn_kernel<T, NH, NB>, 32 * kKv4Warps, kv4_attn_smem<NH, NB>(), T, NH>(a, grid, st, pdl);
 }
-template <class T, int NH>
+template <class T, int NH, int NG>
 cudaError_t prompt_launch(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
   const dim3 grid(static_cast<unsigned>(a.n_seqs) * a.c.n_kv * a.tiles, static_cast<unsigned>(a.splits));
-  return launch_tiles<kv4_prompt_kernel<T, NH>, kKv4PromptThreads, kv4_prompt_smem<NH>(), T, NH>(a, grid, st, pdl);
+  return launch_tiles<kv4_prompt_kernel<T, NH, NG>, kv4_prompt_threads<NG>(), kv4_prompt_smem<NH, NG>(), T, NH>(
+      a, grid, st, pdl);
 }
 
 template <class T, int NH>
 cudaError_t attn_shape(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
-  if (a.tile_cols == kKv4PromptCols) return prompt_launch<T, NH>(a, st, pdl);
+  if (a.tile_cols == 2 * kKv4PromptCols) return prompt_launch<T, NH, 2>(a, st, pdl);
+  if (a.tile_cols == kKv4PromptCols) return prompt_launch<T, NH, 1>(a, st, pdl);
   return a.tile_cols > 8 ? attn_launch<T, NH, 2>(a, st, pdl) : attn_launch<T, NH, 1>(a, st, pdl);
 }
 
@@ -110,19 +112,16 @@ namespace {
 int64_t plan_pages(const Kv4AttnArgs& a) { return std::max(1, (a.max_len + kKv4Page - 1) / kKv4Page); }
 int64_t plan_units(const Kv4AttnArgs& a) { return static_cast<int64_t>(a.n_seqs) * a.c.n_kv * a.tiles; }
 // Splits: at least 32 pages each (8 a warp).  One sequence's splits are alike:
-// one wave of CTAs, four to an SM (131071 positions, 8 kv heads of 128: 47 us,
+// one wave of CTAs, four to an SM (131071 positions, 8 kv heads of 128: 46 us,
 // and 55 us with splits for four waves).  Several sequences differ in length:
-// four waves even that out (32 of 1001 to 16384: 93 us, and 110 us with one).
-// Prompts: only where the tiles leave CTA slots empty, 64 pages each at least
-// (the join reads and writes every column's share: 274 us became 364).
+// four waves even that out (32 of 1001 to 16384: 91 us, and 110 us with one).
+// Prompts: one CTA to an SM, 64 pages each at least (256 rows of 4 heads on 8192
+// positions, 64 tiles: 69 us, and 109 without splits).
 int64_t plan_splits(const Kv4AttnArgs& a, int sms) {
-  const bool prompt = a.tile_cols == kKv4PromptCols;
-  const int64_t ctas = int64_t(sms) * (prompt ? 2 : a.n_seqs == 1 ? 4 : 16), least = prompt ? 64 : 32;
+  const bool prompt = a.tile_cols >= kKv4PromptCols;
+  const int64_t ctas = int64_t(sms) * (prompt ? 1 : a.n_seqs == 1 ? 4 : 16), least = prompt ? 64 : 32;
   return std::max<int64_t>(
       1, std::min<int64_t>(ctas / std::max<int64_t>(1, plan_units(a)), (plan_pages(a) + least - 1) / least));
-}
-uint64_t scratch_of(const Kv4AttnArgs& a, int64_t splits) {
-  return splits <= 1 ? 0 : uint64_t(plan_units(a)) * splits * a.tile_cols * (a.c.d + 4) * sizeof(float);
 }
 }  // namespace
 
@@ -131,11 +130,24 @@ bool kv4_attn_plan(Kv4AttnArgs& a, int sms) {
   a.group_inv = ((uint64_t(1) << 32) + a.group - 1) / a.group;
   const int64_t cols = static_cast<int64_t>(a.max_rows) * a.group;
   if (cols * a.group >= int64_t(1) << 32) return false;
-  // The kernel for prompts takes 128 columns at the price of any: from 65 columns
-  // (16 rows of 4 heads and 128 dims on 2048 positions, 8 sequences: 31 us, and
-  // 40 with tiles of 16; at 64 dims 24 and 17; 32 rows on 8000: 27 and 34).
-  a.tile_cols = cols <= 8 ? 8 : cols <= 64 ? 16 : kKv4PromptCols;
+  // The kernel for prompts takes 128 columns at the price of any; the other one
+  // walks the pages once per 16.  From 65 columns on it is the prompts', and below
+  // where the pages are many (the product of sequences, kv heads, positions, dims
+  // over 128), else its start weighs more.  us, prompts' and other:
+  //   48 columns, 128 dims, 64 Ki: 22 and 26;  16 Ki (64 dims): 18 and 12
+  //   32 columns, 128 dims, 512 Ki: 64 and 85;  64 Ki: 22 and 17
+  //   32 columns,  64 dims, 128 Ki: 34 and 27
+  const int64_t work = int64_t(a.n_seqs) * a.c.n_kv * a.max_len * a.c.d / 128;
+  const bool prompt = cols > 64 || (cols > 32 && work >= 1 << 16) || (cols > 16 && a.c.d == 128 && work >= 1 << 19);
+  a.tile_cols = prompt ? kKv4PromptCols : cols <= 8 ? 8 : 16;
   a.tiles = static_cast<int>((cols + a.tile_cols - 1) / a.tile_cols);
+  // Two groups of columns a CTA share the halves of K and V: where one each would
+  // leave no SM without a CTA (288 tiles of 128 columns on 8192 positions: 147 us,
+  // and 212 with a group a CTA; 144 tiles: 126 and 111).
+  if (prompt && plan_units(a) > sms) {
+    a.tile_cols *= 2;
+    a.tiles = (a.tiles + 1) / 2;
+  }
   const int64_t pages = plan_pages(a), splits = plan_splits(a, sms);
   a.split_pages = static_cast<int>((pages + splits - 1) / splits);
   a.splits = static_cast<int>((pages + a.split_pages - 1) / a.split_pages);
@@ -143,8 +155,13 @@ bool kv4_attn_plan(Kv4AttnArgs& a, int sms) {
   return plan_units(a) <= INT_MAX && a.c.n_kv <= 65535 && int64_t(a.tiles) * a.splits <= 65535 && (a.splits == 1 || cols <= 65535);
 }
 
-uint64_t kv4_attn_scratch(const Kv4AttnArgs& a) { return scratch_of(a, a.splits); }
-uint64_t kv4_attn_scratch_most(const Kv4AttnArgs& a, int sms) { return scratch_of(a, plan_splits(a, sms)); }
+uint64_t kv4_attn_scratch(const Kv4AttnArgs& a) {
+  return a.splits <= 1 ? 0 : uint64_t(plan_units(a)) * a.splits * a.tile_cols * (a.c.d + 4) * sizeof(float);
+}
+uint64_t kv4_attn_scratch_most(int d, int sms) {
+  // (split tiles are no more than the CTAs that plan_splits wants; prompts in pairs are not split)
+  return uint64_t(sms) * std::max(16 * 16, kKv4PromptCols) * (d + 4) * sizeof(float);
+}
 
 cudaError_t kv4_attention(const Kv4AttnArgs& a, cudaStream_t st, bool pdl) {
   if (a.n_rows == 0 || a.n_seqs == 0) return cudaSuccess;

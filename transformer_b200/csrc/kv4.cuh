@@ -1031,17 +1031,17 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
   }
 }
 
-// Joins the splits of each column: one CTA per column, its warps take the
-// splits w, w + 4, .. (8 loads in flight a lane), then meet in warp order.
+// Joins the splits of each column: a warp per column, 8 loads in flight a lane
+// (a CTA per column with its warps on different splits: the same for 32 columns of
+// 74 splits, and 82 us instead of 69 for 256 rows of 4 heads on 8192 positions).
 template <class T, int NH>
 __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ Kv4AttnArgs a) {
-  constexpr int D = 64 * NH, PER = 2 * NH, WARPS = 4, DEEP = 8;
-  __shared__ float s_r[WARPS][D], s_l[WARPS];
+  constexpr int D = 64 * NH, PER = 2 * NH, DEEP = 8;
   pdl_wait();
   pdl_launch();
-  // grid: x = sequence, y = kv head, z = column
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int c = blockIdx.z, tile = c / a.tile_cols;
+  // grid: x = sequence, y = kv head, z = 4 columns
+  const int lane = threadIdx.x & 31;
+  const int c = blockIdx.z * 4 + (threadIdx.x >> 5), tile = c / a.tile_cols;
   Kv4Tile tl;
   if (!kv4_tile(a, blockIdx.x, blockIdx.y, tile, 0, tl) || c >= tl.cols(a)) return;
   const int n = max(1, (kv4_tile_pages(a, tl) + a.split_pages - 1) / a.split_pages);
@@ -1055,11 +1055,11 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ K
   float L = 0.f, r[PER];
 #pragma unroll
   for (int k = 0; k < PER; ++k) r[k] = 0.f;
-  for (int s0 = warp; s0 < n; s0 += WARPS * DEEP) {
+  for (int s0 = 0; s0 < n; s0 += DEEP) {
     float2 ml[DEEP], x[DEEP][NH];
 #pragma unroll
     for (int i = 0; i < DEEP; ++i) {
-      const int s = s0 + WARPS * i;
+      const int s = s0 + i;
       ml[i] = s < n ? *reinterpret_cast<const float2*>(src + s * step + D) : make_float2(-INFINITY, 0.f);
 #pragma unroll
       for (int h = 0; h < NH; ++h)
@@ -1076,19 +1076,14 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ K
       }
     }
   }
+  const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
+  const int row = kv4_row(a, c);
+  T* out = static_cast<T*>(a.out) + static_cast<int64_t>(tl.r0 + row) * a.o_row +
+           static_cast<int64_t>(tl.g * a.group + c - row * a.group) * a.o_head;
 #pragma unroll
-  for (int h = 0; h < NH; ++h) *reinterpret_cast<float2*>(&s_r[warp][64 * h + 2 * lane]) = make_float2(r[2 * h], r[2 * h + 1]);
-  if (lane == 0) s_l[warp] = L;
-  __syncthreads();
-  if (threadIdx.x < D) {
-    const int d = threadIdx.x;
-    L = (s_l[0] + s_l[1]) + (s_l[2] + s_l[3]);
-    const float inv = L > 0.f ? 1.0f / L : (L == 0.f ? 0.f : L);
-    const int row = kv4_row(a, c);
-    static_cast<T*>(a.out)[static_cast<int64_t>(tl.r0 + row) * a.o_row +
-                           static_cast<int64_t>(tl.g * a.group + c - row * a.group) * a.o_head + d] =
-        from_f32<T>(((s_r[0][d] + s_r[1][d]) + (s_r[2][d] + s_r[3][d])) * inv);
-  }
+  for (int h = 0; h < NH; ++h)
+#pragma unroll
+    for (int k = 0; k < 2; ++k) out[64 * h + 2 * lane + k] = from_f32<T>(r[2 * h + k] * inv);
 }
 
 }  // namespace b2d

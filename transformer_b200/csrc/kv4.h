@@ -69,8 +69,8 @@ cudaError_t kv4_read(const Kv4ReadArgs& a, cudaStream_t st);
 // a.part it needs.
 bool kv4_attn_plan(Kv4AttnArgs& a, int sms);
 uint64_t kv4_attn_scratch(const Kv4AttnArgs& a);
-// (planned) The most that it needs at this or a smaller max_len.
-uint64_t kv4_attn_scratch_most(const Kv4AttnArgs& a, int sms);
+// The most that any call on heads of d dims needs.
+uint64_t kv4_attn_scratch_most(int d, int sms);
 cudaError_t kv4_attention(const Kv4AttnArgs& a, cudaStream_t st, bool pdl);
 
 }  // namespace b2d

@@ -1,32 +1,36 @@
 // kv4_prompt.cuh — attention of many query columns over the 4-bit cache on the
 // 5th-generation tensor cores (tcgen05, sm_100a).
 //
-// One CTA takes 128 query columns (row of the sequence, head of the group) of a
-// (sequence, kv head) through tiles of 64 positions:
+// One CTA takes one or two groups of 128 query columns (row of the sequence, head
+// of the group) of a (sequence, kv head) through tiles of 64 positions; for each
+// group
 //   S = Q K^T   M = 128 columns, N = 64 positions, K = d; Q and K in shared memory
 //   O += P V    M = 128 columns, N = d, K = 64 positions; P in tensor memory, V in
 //               shared memory
 // with the halves of kv4.cuh (held values, queries and scores exact, P with 11
-// bits and a factor 2^10).  Its warps have three parts, which meet only on
-// mbarriers:
-//   warps 0-3   softmax: thread r owns column r, lane r of tensor memory
-//   warps 4-7   turn codes to halves, a page of each tile, straight into the
-//               swizzled operands
-//   warp 8      issues the products
-//   (warp 9     waits: registers are granted to pairs of warps)
+// bits and a factor 2^10).  Its warps have parts, which meet only on mbarriers (for
+// two groups):
+//   warps 0-7    softmax: thread r owns column r, lane r % 128 of its group's
+//                tensor memory
+//   warps 8-11   turn K's codes to halves, a page of each tile, straight into the
+//                swizzled operand
+//   warps 12-15  V's
+//   warps 16-17  issue a group's products
 // K, V and S (with P over it) have two buffers each: S of the next tile is made
-// during the softmax of this one, O of the last one too.  Two CTAs share an SM,
-// 256 columns of tensor memory each.
+// during the softmax of this one, O of the last one too.  One CTA to an SM.
 //
 // 4 chunks of 128 to 512 rows on 2049 to 8191 positions, 32 heads over 8 of 128
-// dims (125 GFLOP): 274 us, 455 TFLOP/s.  What bounds it is the chain from a
-// tile's P to the next S in its buffer (some 1600 cycles: hand-overs of 150 to
-// 300 each, both products), and CTAs of unlike length: SMs are idle 40% of the
-// time.  Measured on the same case: tiles of 128 positions with one buffer
-// 296 to 318 us; all eight warps sharing both the softmax and the codes 329;
-// three warps for the codes, so that registers suffice for 64 scores at once,
-// 287; waits that end in a vote or read a timer 322; the positions split in two
-// and joined 364.
+// dims (125 GFLOP): 147 us, 845 TFLOP/s; 288 tiles of equal length 980.  What
+// bounds the latter: per tile and group the softmax has 512 cycles of exponentials
+// on a quarter SM, next to 250 of its other instructions and as many for the
+// codes; both products take 512 of the tensor cores (without the exponentials 130
+// instead of 147 us, without the codes 141, without most of the products 145).
+// The 4 chunks lose another 20% to the longest columns' end.  Measured on the
+// same case: two CTAs to an SM of one group, 205; four warps for K and V
+// together, 166; all 64 scores held at once, 155; one pass with the last
+// maximum that is repeated when that was too small, 158; waits that poll, 147.
+// Before the longest came first, 274: tiles of 128 positions with one buffer 296
+// to 318; all warps sharing softmax and codes 329.
 //
 // The orders are chosen so that a lane's fragments lie together (16 and 8 byte
 // stores without bank conflicts): the dims of K and Q are permuted alike within
@@ -46,17 +50,20 @@
 
 namespace b2d {
 
-constexpr int kKv4PromptCols = 128;  // query columns of a CTA
+constexpr int kKv4PromptCols = 128;  // query columns of a group; a CTA has one or two
 constexpr int kKv4PromptKeys = 64;   // positions of a tile
-constexpr int kKv4PromptThreads = 320;
+template <int NG>
+constexpr __host__ __device__ int kv4_prompt_threads() {
+  return 32 * (4 * NG + 4 + 4 + 2);
+}
 constexpr float kKv4PromptOffset = 10.f, kKv4PromptSlack = 5.f;  // (their sum: P below 2^15)
-constexpr uint32_t kKv4PromptTmem = 256;  // columns: S (P over it) 2 x 64, O d
-template <int NH>
+constexpr uint32_t kKv4PromptTmem = 256;  // columns of a group: S (P over it) 2 x 64, O d
+template <int NH, int NG>
 constexpr __host__ __device__ int kv4_prompt_smem() {
-  // Q, K, V tiles and 1 KB to align; at least 80 KB, so that no more than two CTAs
+  // Q, K, V tiles and 1 KB to align; at least so much that no more groups than two
   // share an SM's tensor memory (a third would wait for it)
-  constexpr int tiles = 3 * NH * 128 * 128 + 1024;
-  return tiles > 80 * 1024 ? tiles : 80 * 1024;
+  constexpr int tiles = (NG + 2) * NH * 128 * 128 + 1024, least = (NG == 1 ? 80 : 120) * 1024;
+  return tiles > least ? tiles : least;
 }
 
 // f16 x f16 -> f32, both operands K-major.
@@ -85,6 +92,32 @@ __device__ __forceinline__ void tmem_load32(uint32_t taddr, uint32_t* r) {
         "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]),
         "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
       : "r"(taddr));
+}
+// Two floats at once.
+__device__ __forceinline__ uint64_t pair_of(uint32_t lo, uint32_t hi) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(hi));
+  return d;
+}
+__device__ __forceinline__ float2 floats_of(uint64_t x) {
+  float2 d;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(x));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ float max3(float a, uint32_t b, uint32_t c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(__uint_as_float(b)), "f"(__uint_as_float(c)));
+  return d;
 }
 __device__ __forceinline__ bool elect_one() {  // of a whole warp: true in one lane
   uint32_t p;
@@ -125,8 +158,8 @@ struct Kv4Frag {
 };
 
 // The sequence that is rank-th from the longest (equal lengths in their order):
-// the longest tiles start first, so that short ones fill the end (the same case:
-// 274 us in the sequences' order).  Whole warp.  More than 32 sequences stay in
+// the longest tiles start first, so that short ones fill the end (4 chunks as
+// above: 205 us, and 274 in the sequences' order).  Whole warp.  More than 32 sequences stay in
 // their order: with so many tiles the last ones are a small part.
 __device__ __forceinline__ int kv4_seq_of_rank(const Kv4AttnArgs& a, int rank) {
   if (a.n_seqs > 32 || a.n_seqs == 1) return rank;
@@ -141,18 +174,19 @@ __device__ __forceinline__ int kv4_seq_of_rank(const Kv4AttnArgs& a, int rank) {
 }
 
 // Grid: x = (rank * kv heads + kv head) * tiles + tile from the last, y = split.
-template <class T, int NH>
-__global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const __grid_constant__ Kv4AttnArgs a) {
+template <class T, int NH, int NG>
+__global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel(const __grid_constant__ Kv4AttnArgs a) {
   constexpr int D = 64 * NH, PB = kv4_page_bytes(D), PAGES = kKv4PromptKeys / kKv4Page;
   extern __shared__ uint8_t kv4_prompt_raw[];
-  // written: K, V, P; products done: S (so K is free), O (so V and P's S are); two buffers each
-  enum { kKFull, kVFull, kPFull, kSDone, kODone, kBars };
+  // written: K, V; of each group, written: P, products done: S (so K is free), O (so V
+  // and P's S are); two buffers each
+  enum { kKFull, kVFull, kPFull, kSDone = kPFull + NG, kODone = kSDone + NG, kBars = kODone + NG };
   __shared__ uint64_t s_bar[kBars][2];
   __shared__ uint32_t s_tmem;
   __shared__ volatile uint32_t s_fail;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
   uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_prompt_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* sk = sq + NH * 128 * 128;  // Q [NH][128 rows][128 B], K [2][NH][64 rows][128 B]
+  uint8_t* sk = sq + NG * NH * 128 * 128;  // Q [NG][NH][128 rows][128 B], K [2][NH][64 rows][128 B]
   uint8_t* sv = sk + NH * 128 * 128;  // V [2][D rows][128 B]
   constexpr int K_BUF = NH * 64 * 128, V_BUF = D * 128;
   pdl_wait();
@@ -166,13 +200,14 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const 
     pdl_launch();
     return;
   }
-  if (warp == 8) tmem_alloc(&s_tmem, kKv4PromptTmem);
+  constexpr int CODES = 4 * NG, ISSUE = CODES + 8;  // the parts' first warps
+  if (warp == ISSUE) tmem_alloc(&s_tmem, NG * kKv4PromptTmem);
   if (tid == 0) {
     for (int i = 0; i < 2 * kBars; ++i) mbar_init(&s_bar[i >> 1][i & 1], i < 2 * kSDone ? 4 : 1);  // 4 warps, or a commit
     fence_mbar_init();
     s_fail = 0u;
   }
-  const int c0 = tl.tile * kKv4PromptCols, cols = tl.cols(a), tiles = (hi - lo + PAGES - 1) / PAGES;
+  const int c0 = tl.tile * NG * kKv4PromptCols, cols = tl.cols(a), tiles = (hi - lo + PAGES - 1) / PAGES;
   // Bounded wait for a barrier's phase of tile i; one that runs out marks the
   // CTA, whose parts then leave their loops.
   auto wait = [&](int which, int i) {
@@ -182,12 +217,13 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const 
   };
 
   // ---- softmax threads: the column and its query ----
-  const int col = c0 + (tid & 127);
-  const bool in = warp < 4 && col < cols;
+  const int groups = min(NG, (cols - c0 + kKv4PromptCols - 1) / kKv4PromptCols);
+  const int col = c0 + tid, gr = warp >> 2;
+  const bool in = warp < CODES && col < cols;
   const int row = in && tl.rows > 1 ? kv4_row(a, col) : 0, head = in ? col - row * a.group : 0;
   float up = a.scale_log2;
-  if (warp < 4) {
-    // halves, dims in the codes' order, to row tid of sq
+  if (warp < CODES) {
+    // halves, dims in the codes' order, to row tid of its group's Q
     const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(tl.r0 + row) * a.q_row +
                  static_cast<int64_t>(tl.g * a.group + head) * a.q_head;
     const bool vec = aligned16(a.q, a.q_row, a.q_head, sizeof(T));
@@ -224,7 +260,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const 
             f[4 * k + s] = s & 1 ? pack_half2(bf16_hi(x) * down, bf16_hi(y) * down)
                                  : pack_half2(bf16_lo(x) * down, bf16_lo(y) * down);
         }
-      uint8_t* dst = sq + (b >> 2) * 16384 + tid * 128;
+      uint8_t* dst = sq + (gr * NH + (b >> 2)) * 16384 + (tid & 127) * 128;
       const int c = (b & 3) * 2;
       *reinterpret_cast<uint4*>(dst + ((c ^ (tid & 7)) << 4)) = make_uint4(f[0], f[1], f[2], f[3]);
       *reinterpret_cast<uint4*>(dst + (((c + 1) ^ (tid & 7)) << 4)) = make_uint4(f[4], f[5], f[6], f[7]);
@@ -236,19 +272,23 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const 
   __syncthreads();
   tc_fence_after();
   pdl_launch();  // (every CTA that runs now holds its tensor memory)
-  const uint32_t t_s = s_tmem, t_o = t_s + 128;
+  // this group's tensor memory (groups of the issuing warps: below)
+  auto t_s_of = [&](int g) { return s_tmem + 128 * g; };
+  auto t_o_of = [&](int g) { return s_tmem + 128 * NG + D * g; };
 
-  if (warp == 8) {  // ---- products ----
+  if (warp >= ISSUE) {  // ---- products: a warp a group ----
     // (the whole warp walks along, so that descriptors stay in uniform registers)
+    const int g = warp - ISSUE;
+    const uint32_t t_s = t_s_of(g), t_o = t_o_of(g);
     const bool leader = elect_one();
-    const uint32_t q0 = smem_addr(sq), k0 = smem_addr(sk), v0 = smem_addr(sv);
+    const uint32_t q0 = smem_addr(sq) + g * NH * 16384, k0 = smem_addr(sk), v0 = smem_addr(sv);
     auto poll = [&](int which, int i) {
       if (kv4_poll(&s_bar[which][i & 1], static_cast<uint32_t>(i >> 1) & 1u)) return true;
       s_fail = 1u;
       return false;
     };
     auto issue_s = [&](int i) {
-      if (!poll(kKFull, i) || (i >= 2 && !poll(kODone, i - 2))) return false;
+      if (!poll(kKFull, i) || (i >= 2 && !poll(kODone + g, i - 2))) return false;
       tc_fence_after();
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
@@ -256,13 +296,13 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const 
         const uint64_t kd = sdesc_kmajor_sw128(k0 + (i & 1) * K_BUF + (k >> 2) * 8192 + (k & 3) * 32);
         if (leader) tc_mma_bf16(t_s + 64 * (i & 1), qd, kd, idesc_f16_f32(128, 64), k > 0);
       }
-      if (leader) tc_commit(&s_bar[kSDone][i & 1]);
+      if (leader) tc_commit(&s_bar[kSDone + g][i & 1]);
       return true;
     };
-    bool ok = tiles > 0 && issue_s(0);
+    bool ok = g < groups && tiles > 0 && issue_s(0);
     for (int i = 0; ok && i < tiles; ++i) {
       if (i + 1 < tiles) ok = issue_s(i + 1);
-      ok = ok && poll(kVFull, i) && poll(kPFull, i);
+      ok = ok && poll(kVFull, i) && poll(kPFull + g, i);
       if (!ok) break;
       tc_fence_after();
 #pragma unroll
@@ -270,15 +310,13 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const 
         const uint64_t vd = sdesc_kmajor_sw128(v0 + (i & 1) * V_BUF + k * 32);
         if (leader) tc_mma_f16_ts(t_o, t_s + 64 * (i & 1) + 8 * k, vd, idesc_f16_f32(128, D), i > 0 || k > 0);
       }
-      if (leader) tc_commit(&s_bar[kODone][i & 1]);
+      if (leader) tc_commit(&s_bar[kODone + g][i & 1]);
     }
-  } else if (warp == 9) {
-  } else if (warp >= 4) {  // ---- codes to halves ----
+  } else if (warp >= CODES) {  // ---- codes to halves ----
     const int32_t* table = a.c.table + tl.seq * a.c.table_ld;
     const uint8_t* pool = a.c.pool + static_cast<int64_t>(tl.g) * PB;
     const int64_t block_bytes = static_cast<int64_t>(a.c.n_kv) * PB;
-    const int seen = kv4_limit(a, tl, min(cols, c0 + kKv4PromptCols) - 1);  // positions that any column sees
-    const int mine = warp - 4;  // this warp's page of a tile
+    const int mine = warp & 3;  // this warp's page of a tile
     // the block of this warp's page of tile i, as the table has it
     auto block_of = [&](int i) {
       const int pg = lo + i * PAGES + mine;
@@ -290,111 +328,127 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const 
       if (lane == 0 && lo + i * PAGES + mine < hi) kv4_error(a.c.status, kKv4BadTable);
       return nullptr;
     };
-    auto load_k = [&](Kv4Frag<NH>& kf, const uint8_t* page) {
-#pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        kf.code[h] = make_uint4(0u, 0u, 0u, 0u);
-        kf.scale[h] = 0u;
-        if (page != nullptr) {
-          kf.code[h] = __ldg(reinterpret_cast<const uint4*>(page) + h * 32 + lane);
-          kf.scale[h] = __ldg(reinterpret_cast<const uint16_t*>(page + 8 * D) + h * 32 + lane);
-        }
-      }
-    };
-    auto load_v = [&](Kv4Frag<NH>& vf, const uint8_t* page) {
-#pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        vf.code[h] = make_uint4(0u, 0u, 0u, 0u);
-        vf.scale[h] = 0u;
-        if (page != nullptr) {
-          vf.code[h] = __ldg(reinterpret_cast<const uint4*>(page + 9 * D) + h * 32 + lane);
-          vf.scale[h] = __ldg(reinterpret_cast<const uint32_t*>(page + 17 * D) + (h * 4 + (gid >> 1)) * 4 + tig);
-        }
-      }
-    };
-    // this lane's rows of the K tile: slots gid and gid + 8 of a page are its columns r, r + 2
-    const int r = 16 * mine + 4 * (gid >> 1) + (gid & 1), vrow = kv4_perm(gid);
-    uint8_t* const k_to = sk + r * 128;
-    uint8_t* const v_to = sv + vrow * 128 + (((mine * 2 + (tig >> 1)) ^ vrow) << 4) + (tig & 1) * 8;
+    // Tile i, whose page is in f; f takes tile i + 2's, so that a load has a tile's
+    // time to arrive (block: its number in the pool, loaded a tile before).
     int block = block_of(2);
-    // Tile i, whose page is in kf and vf; they take tile i + 2's, so that a load has
-    // a tile's time to arrive (block: its number in the pool, loaded a tile before).
-    auto tile = [&](int i, Kv4Frag<NH>& kf, Kv4Frag<NH>& vf) {
-      if (i >= 2 && !wait(kSDone, i - 2)) return false;
+    Kv4Frag<NH> frag[2];
+    auto walk = [&](auto&& load, auto&& convert) {
 #pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        const uint32_t s0 = kv4_scales(kf.scale[h], 0x4040), s1 = kv4_scales(kf.scale[h], 0x4141);
-        uint32_t v[4];
-        uint8_t* d0 = k_to + (i & 1) * K_BUF + h * 8192;
-        uint8_t* d1 = d0 + 2 * 128;
-        kv4_values(kf.code[h].x, s0, v);
-        *reinterpret_cast<uint4*>(d0 + (((2 * tig) ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-        kv4_values(kf.code[h].y, s0, v);
-        *reinterpret_cast<uint4*>(d0 + (((2 * tig + 1) ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-        kv4_values(kf.code[h].z, s1, v);
-        *reinterpret_cast<uint4*>(d1 + (((2 * tig) ^ ((r + 2) & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-        kv4_values(kf.code[h].w, s1, v);
-        *reinterpret_cast<uint4*>(d1 + (((2 * tig + 1) ^ ((r + 2) & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_bar[kKFull][i & 1]);
-      const uint8_t* page = page_at(i + 2, block);
-      block = block_of(i + 3);
-      load_k(kf, page);
-      if (i >= 2 && !wait(kODone, i - 2)) return false;
-      // slots past the last position seen may never have been written: no scale
-      const int left = seen - (lo + i * PAGES + mine) * kKv4Page;
-      uint32_t keep = 0xFFFFFFFFu;
-      if (left < kKv4Page) {
-        keep = 0u;
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (2 * tig + 8 * (j >> 1) + (j & 1) < left) keep |= 0xFFu << (8 * j);
-      }
-#pragma unroll
-      for (int h = 0; h < NH; ++h) {
-        uint8_t* dst = v_to + (i & 1) * V_BUF + h * 8192;
-        const uint32_t sc = vf.scale[h] & keep;
-        const uint32_t s0 = kv4_scales(sc, 0x4140), s1 = kv4_scales(sc, 0x4342);
-        uint32_t x[4], y[4];
-        kv4_values(vf.code[h].x, s0, x);
-        kv4_values(vf.code[h].z, s1, y);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint2*>(dst + 8 * j * 128) = make_uint2(x[j], y[j]);
-        kv4_values(vf.code[h].y, s0, x);
-        kv4_values(vf.code[h].w, s1, y);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) *reinterpret_cast<uint2*>(dst + (32 + 8 * j) * 128) = make_uint2(x[j], y[j]);
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&s_bar[kVFull][i & 1]);
-      load_v(vf, page);
-      return true;
+      for (int i = 0; i < 2; ++i) load(frag[i], page_at(i, block_of(i)));
+      auto one = [&](int i, Kv4Frag<NH>& f) {
+        if (!convert(i, f)) return false;
+        const uint8_t* page = page_at(i + 2, block);
+        block = block_of(i + 3);
+        load(f, page);
+        return true;
+      };
+      for (int i = 0; i < tiles; i += 2)
+        if (!one(i, frag[0]) || (i + 1 < tiles && !one(i + 1, frag[1]))) break;
     };
-    Kv4Frag<NH> kf[2], vf[2];
+    // the tile's buffer is written: for the products, and told by one lane
+    auto written = [&](int which, int i) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&s_bar[which][i & 1]);
+    };
+    if (warp < CODES + 4) {
+      // this lane's rows of the K tile: slots gid and gid + 8 of a page are its columns r, r + 2
+      const int r = 16 * mine + 4 * (gid >> 1) + (gid & 1);
+      uint8_t* const k_to = sk + r * 128;
+      walk(
+          [&](Kv4Frag<NH>& kf, const uint8_t* page) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const uint8_t* page = page_at(i, block_of(i));
-      load_k(kf[i], page);
-      load_v(vf[i], page);
+            for (int h = 0; h < NH; ++h) {
+              kf.code[h] = make_uint4(0u, 0u, 0u, 0u);
+              kf.scale[h] = 0u;
+              if (page != nullptr) {
+                kf.code[h] = __ldg(reinterpret_cast<const uint4*>(page) + h * 32 + lane);
+                kf.scale[h] = __ldg(reinterpret_cast<const uint16_t*>(page + 8 * D) + h * 32 + lane);
+              }
+            }
+          },
+          [&](int i, const Kv4Frag<NH>& kf) {
+            for (int g = 0; g < groups; ++g)
+              if (i >= 2 && !wait(kSDone + g, i - 2)) return false;
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+              const uint32_t s0 = kv4_scales(kf.scale[h], 0x4040), s1 = kv4_scales(kf.scale[h], 0x4141);
+              uint32_t v[4];
+              uint8_t* d0 = k_to + (i & 1) * K_BUF + h * 8192;
+              uint8_t* d1 = d0 + 2 * 128;
+              kv4_values(kf.code[h].x, s0, v);
+              *reinterpret_cast<uint4*>(d0 + (((2 * tig) ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+              kv4_values(kf.code[h].y, s0, v);
+              *reinterpret_cast<uint4*>(d0 + (((2 * tig + 1) ^ (r & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+              kv4_values(kf.code[h].z, s1, v);
+              *reinterpret_cast<uint4*>(d1 + (((2 * tig) ^ ((r + 2) & 7)) << 4)) = make_uint4(v[0], v[1], v[2], v[3]);
+              kv4_values(kf.code[h].w, s1, v);
+              *reinterpret_cast<uint4*>(d1 + (((2 * tig + 1) ^ ((r + 2) & 7)) << 4)) =
+                  make_uint4(v[0], v[1], v[2], v[3]);
+            }
+            written(kKFull, i);
+            return true;
+          });
+    } else {
+      const int seen = kv4_limit(a, tl, min(cols, c0 + NG * kKv4PromptCols) - 1);  // positions that any column sees
+      const int vrow = kv4_perm(gid);
+      uint8_t* const v_to = sv + vrow * 128 + (((mine * 2 + (tig >> 1)) ^ vrow) << 4) + (tig & 1) * 8;
+      walk(
+          [&](Kv4Frag<NH>& vf, const uint8_t* page) {
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+              vf.code[h] = make_uint4(0u, 0u, 0u, 0u);
+              vf.scale[h] = 0u;
+              if (page != nullptr) {
+                vf.code[h] = __ldg(reinterpret_cast<const uint4*>(page + 9 * D) + h * 32 + lane);
+                vf.scale[h] = __ldg(reinterpret_cast<const uint32_t*>(page + 17 * D) + (h * 4 + (gid >> 1)) * 4 + tig);
+              }
+            }
+          },
+          [&](int i, const Kv4Frag<NH>& vf) {
+            for (int g = 0; g < groups; ++g)
+              if (i >= 2 && !wait(kODone + g, i - 2)) return false;
+            // slots past the last position seen may never have been written: no scale
+            const int left = seen - (lo + i * PAGES + mine) * kKv4Page;
+            uint32_t keep = 0xFFFFFFFFu;
+            if (left < kKv4Page) {
+              keep = 0u;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (2 * tig + 8 * (j >> 1) + (j & 1) < left) keep |= 0xFFu << (8 * j);
+            }
+#pragma unroll
+            for (int h = 0; h < NH; ++h) {
+              uint8_t* dst = v_to + (i & 1) * V_BUF + h * 8192;
+              const uint32_t sc = vf.scale[h] & keep;
+              const uint32_t s0 = kv4_scales(sc, 0x4140), s1 = kv4_scales(sc, 0x4342);
+              uint32_t x[4], y[4];
+              kv4_values(vf.code[h].x, s0, x);
+              kv4_values(vf.code[h].z, s1, y);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) *reinterpret_cast<uint2*>(dst + 8 * j * 128) = make_uint2(x[j], y[j]);
+              kv4_values(vf.code[h].y, s0, x);
+              kv4_values(vf.code[h].w, s1, y);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) *reinterpret_cast<uint2*>(dst + (32 + 8 * j) * 128) = make_uint2(x[j], y[j]);
+            }
+            written(kVFull, i);
+            return true;
+          });
     }
-    for (int i = 0; i < tiles; i += 2)
-      if (!tile(i, kf[0], vf[0]) || (i + 1 < tiles && !tile(i + 1, kf[1], vf[1]))) break;
-  } else {  // ---- softmax ----
-    const uint32_t t_lane = static_cast<uint32_t>(warp * 32) << 16;
+  } else if (gr < groups) {  // ---- softmax ----
+    const uint32_t t_s = t_s_of(gr), t_o = t_o_of(gr), t_lane = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const int lim = in ? kv4_limit(a, tl, col) : 0;  // positions this column sees
-    const int all_see = kv4_limit(a, tl, c0);        // that all do
+    const int all_see = kv4_limit(a, tl, c0 + gr * kKv4PromptCols);  // that all do
     float m = -INFINITY, l = 0.f;  // maximum of the scores before their scale, as used; sum of p
     for (int i = 0; i < tiles; ++i) {
-      if (!wait(kSDone, i)) break;
+      if (!wait(kSDone + gr, i)) break;
       tc_fence_after();
       const int tile_page = lo + i * PAGES, at = tile_page * kKv4Page;
       const uint32_t t_mine = t_s + t_lane + 64 * (i & 1);
       const bool edge = at + kKv4PromptKeys > all_see || tile_page + PAGES > hi;
       const int left = min(lim, hi * kKv4Page) - at;  // of the tile, those this column sees
-      uint32_t s[32];
+      uint32_t s[32];  // half of the scores at a time: the second, the first, the second again
       auto scores = [&](int c0) {
         tmem_load32(t_mine + c0, s);
         tmem_wait_ld();
@@ -409,7 +463,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const 
       for (int c0 = 32; c0 >= 0; c0 -= 32) {
         scores(c0);
 #pragma unroll
-        for (int c = 0; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], __uint_as_float(s[c]));
+        for (int c = 0; c < 32; c += 2) mx[(c >> 1) & 3] = max3(mx[(c >> 1) & 3], s[c], s[c + 1]);
       }
       const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
       // (from -infinity too; not for a column that sees nothing)
@@ -419,7 +473,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const 
         m = mn;
         l *= f;
         if (i > 0) {
-          if (!wait(kODone, i - 1)) break;
+          if (!wait(kODone + gr, i - 1)) break;
           tc_fence_after();
 #pragma unroll
           for (int c = 0; c < D; c += 16) {
@@ -433,27 +487,30 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const 
         }
       }
       const float sub = fmaf(m == -INFINITY ? 0.f : -m, up, kKv4PromptOffset);
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
+      const uint64_t up2 = pair_of(__float_as_uint(up), __float_as_uint(up));
+      const uint64_t sub2 = pair_of(__float_as_uint(sub), __float_as_uint(sub));
+      uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
         if (c > 0) scores(c);
         uint32_t p[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const float x = exp2_fast(fmaf(__uint_as_float(s[2 * k]), up, sub));
-          const float y = exp2_fast(fmaf(__uint_as_float(s[2 * k + 1]), up, sub));
-          sum[k & 3] += x + y;
+          const float2 e = floats_of(fma2(pair_of(s[2 * k], s[2 * k + 1]), up2, sub2));
+          const float x = exp2_fast(e.x), y = exp2_fast(e.y);
+          sum[k & 1] = add2(sum[k & 1], pair_of(__float_as_uint(x), __float_as_uint(y)));
           p[k] = pack_half2(x, y);
         }
         tmem_store16(t_mine + (c >> 1), p);  // over scores that have been taken
       }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+      const float2 s0 = floats_of(add2(sum[0], sum[1]));
+      l += s0.x + s0.y;
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&s_bar[kPFull][i & 1]);
+      if (lane == 0) mbar_arrive(&s_bar[kPFull + gr][i & 1]);
     }
-    if (tiles > 0) wait(kODone, tiles - 1);
+    if (tiles > 0) wait(kODone + gr, tiles - 1);
     tc_fence_after();
 
     // ---- the column's result ----
@@ -500,7 +557,7 @@ __global__ void __launch_bounds__(kKv4PromptThreads, 2) kv4_prompt_kernel(const 
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == 8) tmem_dealloc(s_tmem, kKv4PromptTmem);
+  if (warp == ISSUE) tmem_dealloc(s_tmem, NG * kKv4PromptTmem);
 }
 
 }  // namespace b2d
