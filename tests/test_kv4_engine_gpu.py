@@ -298,3 +298,29 @@ def test_rules_change_nothing_when_they_say_nothing(engine_tiny_batched):
         rid = cb.submit(p, 40, **kw)
         out.append(cb.run()[rid])
     assert out[0] == out[1] == out[2]
+
+
+def test_a_rule_that_raises_ends_its_request_alone(engine_tiny_batched):
+    from transformer_b200.config import CONFIG_TINY as cfg
+    rng = np.random.default_rng(8)
+    prompts = [rng.integers(0, cfg.vocab_size, n) for n in (9, 17, 4)]
+    plain = ContinuousBatcher(engine_tiny_batched, 3, 40)
+    ids = [plain.submit(p, 20) for p in prompts]
+    alone = [plain.run()[i] for i in ids]
+
+    def at_once(out):
+        raise KeyError("no rule")
+
+    def later(out):
+        return [5] if len(out) < 3 else [cfg.vocab_size]
+
+    cb = ContinuousBatcher(engine_tiny_batched, 3, 40)
+    ids = [cb.submit(prompts[0], 20), cb.submit(prompts[1], 20, allowed=at_once),
+           cb.submit(prompts[2], 20, allowed=later)]
+    got = cb.run()
+    assert got[ids[0]] == alone[0] and got[ids[1]] == [] and got[ids[2]] == [5, 5, 5]
+    assert set(cb.errors) == set(ids[1:])
+    assert isinstance(cb.errors[ids[1]], KeyError) and isinstance(cb.errors[ids[2]], ValueError)
+    assert cb.pages.n_free == 40
+    again = cb.submit(prompts[1], 20)
+    assert cb.run()[again] == alone[1]

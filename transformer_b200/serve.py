@@ -190,6 +190,7 @@ class ContinuousBatcher:
         self.slots: list[Request | None] = [None] * max_batch
         self.waiting: collections.deque[Request] = collections.deque()
         self.finished: dict[int, list] = {}
+        self.errors: dict[int, Exception] = {}  # of requests that their ``allowed`` function ended
         self._next_rid = 0
         self._admit_tick = 0
         self._hist_cap = hist_cap or self.ctx
@@ -208,7 +209,9 @@ class ContinuousBatcher:
         subtracted from the logits of tokens it has generated, once and times
         their count; ``logit_bias`` {token: value} is added; ``allowed`` are the
         only token ids it may draw, or a function of the list of its generated
-        tokens that gives them (none: the request ends)."""
+        tokens that gives them (none: the request ends; so it does when the
+        function raises or names a token that is none, and ``errors[id]`` has
+        the exception)."""
         prompt = np.asarray(prompt, dtype=np.int32).reshape(-1)
         if prompt.size == 0:
             raise ValueError("empty prompt")
@@ -708,7 +711,12 @@ class ContinuousBatcher:
                 k = ints[1, i] = len(r.logit_bias)
                 bias_ids[i, :k], bias[i, :k] = list(r.logit_bias), list(r.logit_bias.values())
             if r.allowed is not None:
-                ids = self._allowed_ids(r.allowed(list(r.out))) if callable(r.allowed) else r.allowed
+                ids = r.allowed
+                if callable(ids):
+                    try:
+                        ids = self._allowed_ids(ids(list(r.out)))
+                    except Exception as e:  # of the caller's code; the batch's other requests go on
+                        self.errors[r.rid], ids = e, np.zeros(0, np.int64)
                 if not ids.size:
                     ended.add(i)
                 allow[i] = 0
