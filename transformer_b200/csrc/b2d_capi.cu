@@ -1025,6 +1025,7 @@ b2d_status run_rows(b2d_model* m, b2d_ws* ws, const int32_t* tok, const int32_t*
   if (kv4) {
     kt = kv4_attn_args(ws, pos, table, pa.table_ld, bps, num_blocks, batch, pa.table_ld == 0 && batch > 1, 0, cache);
     if (!b2d::kv4_attn_plan(kt, m->grid) || b2d::kv4_attn_scratch(kt) > ws->kv4_part_bytes) return B2D_ERR_UNSUPPORTED;
+    kt.early = !prefill;  // a decode row writes its position only
     ka.q = ws->qkv;
     ka.k = ws->qkv + c.n_heads * 64;
     ka.v = ws->qkv + (c.n_heads + c.n_kv_heads) * 64;

@@ -732,15 +732,19 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
     fence_mbar_init();
   }
   __syncwarp();
-  pdl_wait();
+  bool after = !a.early;  // the kernel before has ended
+  if (after) pdl_wait();
   pdl_launch();
   Kv4Tile tl;
   // grid: x = sequence, y = kv head, z = tile + tiles * split
   const int split = a.tiles == 1 ? blockIdx.z : blockIdx.z / a.tiles;
-  if (!kv4_tile(a, blockIdx.x, blockIdx.y, blockIdx.z - split * a.tiles, split, tl)) return;
-  const int pages = kv4_tile_pages(a, tl);
-  const int lo = tl.split * a.split_pages, hi = min(pages, lo + a.split_pages);
-  if (lo >= hi && tl.split > 0) return;  // (the first split always answers)
+  const bool work = kv4_tile(a, blockIdx.x, blockIdx.y, blockIdx.z - split * a.tiles, split, tl);
+  const int pages = work ? kv4_tile_pages(a, tl) : 0;
+  const int lo = split * a.split_pages, hi = min(pages, lo + a.split_pages);
+  if (!work || (lo >= hi && split > 0)) {  // (the first split always answers)
+    if (!after) pdl_wait();
+    return;
+  }
   const int c0 = tl.tile * COLS, cols = tl.cols(a);
 
   // ---- the warp's pages: the k-th is lo + warp + W k ----
@@ -785,9 +789,14 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
 #pragma unroll
   for (int st = 0; st < kKv4Ahead; ++st) {
     const int next = load_id(st + 1);
+    if (!after && st == steps - 1) {  // the sequence's last page may be in a warp's last step
+      pdl_wait();
+      after = true;
+    }
     issue(st, id);
     id = next;
   }
+  if (!after) pdl_wait();
 
   // query fragments: column gid of each block, dims 64h + 16 tig .. in the codes' order
   uint32_t qf[NB][NH][8];
