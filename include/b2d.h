@@ -389,7 +389,8 @@ typedef struct {
   void* pool;
   const int32_t* table; /* [table_rows][blocks_per_seq]: block of positions 16i.. of each sequence */
   uint32_t* status;     /* device word (or NULL) that the first bad input sets: 0x202 a position,
-                           length or row range, 0x203 a table row or entry; never cleared here */
+                           length or row range, 0x203 a table row or entry, 0x10D a wait in a
+                           kernel that ran out; never cleared here */
   int32_t n_kv_heads, d_head, num_blocks, blocks_per_seq, table_rows;
   int32_t device;
 } b2d_kv4_cache;
@@ -412,7 +413,7 @@ typedef struct {
  * `interleaved`), writes the turned q to q_out, and writes k (turned) and v to
  * the rows' positions in the cache.  The codes are those of the exact rotation
  * of the given numbers (the kernel carries it to 47 bits).  A position that
- * two rows of a call name receives either row's dims, in no particular order.
+ * two rows of a call name gets bytes of both: finite, else undefined.
  * Rows whose position lies past the table or the angles are skipped and set
  * the status.
  */

@@ -182,6 +182,27 @@ def test_append_skips_idle_and_bad_rows(cuda):
     assert torch.count_nonzero(a) == 0 and torch.count_nonzero(b) == 0 and int(status.item()) == 0x203
 
 
+def test_append_two_rows_at_one_position(cuda):
+    """Bytes of both: finite, within the larger row's reach; other rows as alone."""
+    rng = np.random.default_rng(41)
+    n, n_kv, d = 6, 3, 128
+    gen = torch.Generator().manual_seed(5)
+    k = torch.randn(n, n_kv, d, generator=gen).to(cuda)
+    v = 50 * torch.randn(n, n_kv, d, generator=gen).to(cuda)
+    pos, table = i32([0, 7, 7, 7, 20, 3], cuda), i32(rng.permutation(4)[None, :2], cuda)
+    seq = i32([0] * n, cuda)
+    pool = new_kv4_pool(4, n_kv, d)
+    kv4_append(pool, k, v, pos, table, seq=seq)
+    got = kv4_read(pool, pos, table, seq=seq, dtype=torch.float32)
+    for x, y in zip((k, v), got):
+        assert torch.isfinite(y).all() and float(y[1:4].abs().max()) <= 1.15 * float(x[1:4].abs().max())
+    keep = torch.tensor([0, 4, 5], device=cuda)
+    alone = new_kv4_pool(4, n_kv, d)
+    kv4_append(alone, k[keep], v[keep], pos[keep], table, seq=seq[:3])
+    for y, z in zip(got, kv4_read(alone, pos[keep], table, seq=seq[:3], dtype=torch.float32)):
+        assert torch.equal(y[keep], z)
+
+
 def test_append_turns_q_in_place_and_unaligned_rows(cuda):
     """q_out = q gives what a separate q_out gives; rows that start off 16
     bytes (a view one element in) and strided heads give the same."""

@@ -123,7 +123,7 @@ def kv4_append(pool, k, v, pos, table, *, seq=None, q=None, q_out=None, cos=None
     turn (pairs i, i + r / 2; with ``interleaved`` 2i, 2i + 1); None: no
     rotation.  ``q`` [n, heads, d] is turned alike into ``q_out`` (default: a
     new tensor; may be ``q``; a float32 ``q`` also into bf16 or fp16), which is
-    returned.  Two rows at one position: the cache gets dims of either."""
+    returned.  Two rows of a call at one position leave bytes of both there."""
     c, dev, _, table_rows, n_kv, d = _cache(pool, table, status)
     n = pos.numel()
     shape = (n, n_kv, d)
