@@ -182,6 +182,33 @@ def test_append_skips_idle_and_bad_rows(cuda):
     assert torch.count_nonzero(a) == 0 and torch.count_nonzero(b) == 0 and int(status.item()) == 0x203
 
 
+@pytest.mark.parametrize("dtype,heads,n_kv,d,rotary,interleaved", [
+    ("bf16", 16, 4, 64, 64, False), ("f16", 7, 3, 128, 64, True), ("f32", 6, 2, 128, 100, False), ("bf16", 3, 3, 64, 0, False)])
+def test_append_and_read_of_many_rows(cuda, dtype, heads, n_kv, d, rotary, interleaved):
+    """A pass of many rows (another split of the work) holds and gives what small ones do."""
+    n, t = 1100, TYPES[dtype]
+    rng = np.random.default_rng(d + heads)
+    gen = torch.Generator().manual_seed(d)
+    q, k, v = (torch.randn(n, h, d, generator=gen).to(t).to(cuda) for h in (heads, n_kv, n_kv))
+    bps = (n + 15) // 16
+    table = i32(rng.permutation(2 * bps)[:bps][None], cuda)
+    pos, seq = i32(rng.permutation(n), cuda), i32([0] * n, cuda)
+    ang = torch.randn(n, max(1, rotary // 2), generator=gen)
+    kw = dict(cos=ang.cos().to(cuda), sin=ang.sin().to(cuda), interleaved=interleaved) if rotary else {}
+    pools = [new_kv4_pool(2 * bps, n_kv, d, cuda) for _ in range(2)]
+    whole = kv4_append(pools[0], k, v, pos, table, seq=seq, q=q, **kw)
+    got = kv4_read(pools[0], pos, table, seq=seq, dtype=t)
+    for lo in range(0, n, 300):
+        c = slice(lo, min(n, lo + 300))
+        part = kv4_append(pools[1], k[c], v[c], pos[c], table, seq=seq[c], q=q[c], **kw)
+        assert torch.equal(part, whole[c])
+    assert torch.equal(*pools)
+    for lo in range(0, n, 300):
+        c = slice(lo, min(n, lo + 300))
+        for x, y in zip(got, kv4_read(pools[1], pos[c], table, seq=seq[c], dtype=t)):
+            assert torch.equal(x[c], y)
+
+
 def test_append_two_rows_at_one_position(cuda):
     """Bytes of both: finite, within the larger row's reach; other rows as alone."""
     rng = np.random.default_rng(41)

@@ -17,9 +17,11 @@ namespace {
 template <class T, class TQ>
 cudaError_t append_typed(const Kv4AppendArgs& a, cudaStream_t st, bool pdl) {
   // Many rows: a warp takes a whole row, so its addresses and angles are worked
-  // out once (10242 rows: 98 us with the read-back, 108 with four warps a row);
-  // few: a block per batch of heads, one head a thread (512 rows: 7.7 us).
-  const bool many = a.n_rows >= 2048;
+  // out once (10242 rows of 48 heads of 128: 98 us with the read-back, 108 with
+  // four warps a row); few: a block per batch of heads, one head a thread.  Rows
+  // of 48 heads of 128, of 24 of 64 (us, few and many): 512 10.2 and 15.6, 5.7 and
+  // 5.7; 1024 16.8 and 17.0, 9.3 and 7.4; 2000 30.3 and 20.8, 15.8 and 8.4.
+  const bool many = a.n_rows >= 8 * a.c.d;
   const int threads = many ? 32 : kKv4AppendThreads;
   const int slices = threads / (a.c.d / 8);
   const unsigned batches = many ? 1u : static_cast<unsigned>((a.n_heads + slices - 1) / slices + 2);
@@ -101,7 +103,7 @@ cudaError_t kv4_read(const Kv4ReadArgs& a, cudaStream_t st) {
   if (a.n_rows == 0) return cudaSuccess;
   const int slices = 128 / (a.c.d / 8);
   const dim3 grid(static_cast<unsigned>(a.n_rows),
-                  a.n_rows >= 2048 ? 1u : static_cast<unsigned>(std::min(65535, (2 * a.c.n_kv + slices - 1) / slices))),
+                  a.n_rows >= 1024 ? 1u : static_cast<unsigned>(std::min(65535, (2 * a.c.n_kv + slices - 1) / slices))),
       block(128);
   if (a.dtype == B2D_F32) return launch(kv4_read_kernel<float>, grid, block, 0, st, false, a);
   if (a.dtype == B2D_F16) return launch(kv4_read_kernel<__half>, grid, block, 0, st, false, a);
