@@ -6,11 +6,12 @@
 // The lists are short beside the vocabulary: a bit per token in `touched` says
 // where counts and bias places need a look.  Counts are integers and a bias
 // place is the largest index, so no result depends on an order.
-// 256 rows of 32000 with masks, 511 tokens of history and 16 biases: 16.0 us, 4.2 TB/s
-// (67 MB at the copy rate: 10.2); 65 rows of 100003 with 4096 of history: 19.8 us,
+// 256 rows of 32000 with masks, 511 tokens of history and 16 biases: 15.1 us, 4.4 TB/s
+// (67 MB at the copy rate: 10.2); 65 rows of 100003 with 4096 of history: 18.9 us,
 // since each of a row's 25 CTAs looks through all of the history.  Bound by the
-// CTA's chain of list, count and store, five CTAs to an SM; three ids of a list in
-// flight 16.5 and 19.2, four 17.6 and 20.6, four CTAs 18.1 and 21.0.
+// CTA's chain of list, count and store, five CTAs to an SM.  Measured against 16.0
+// and 19.8: three ids of a list in flight 16.5 and 19.2, four 17.6 and 20.6, four
+// CTAs 18.1 and 21.0, slices of 8192 by 512 threads 16.3 and 17.6.
 #include <algorithm>
 
 #include "b2d_host.h"
@@ -28,9 +29,11 @@ constexpr int kLogitsIds = 2;  // ids of a list a thread has in flight
 
 __global__ void __launch_bounds__(kLogitsThreads, 5) adjust_logits_kernel(const __grid_constant__ b2d_logits_rules a,
                                                                        int slice) {
-  __shared__ __align__(16) uint32_t touched[kLogitsSlice / 32];
-  __shared__ __align__(16) uint32_t count[kLogitsSlice];
-  __shared__ __align__(16) uint32_t place[kLogitsSlice];  // 1 + index of the bias that holds
+  // (the bits, which every token looks at, first: 15.1 and 18.9 us, and 16.0 and 19.8 behind the rest)
+  __shared__ __align__(16) uint32_t lists_mem[kLogitsSlice / 32 + 2 * kLogitsSlice];
+  uint32_t* touched = lists_mem;
+  uint32_t* count = touched + kLogitsSlice / 32;
+  uint32_t* place = count + kLogitsSlice;  // 1 + index of the bias that holds
   const int tid = threadIdx.x, lane = tid & 31;
   const int row = blockIdx.y, v0 = blockIdx.x * slice;
   const int n = min(slice, a.vocab - v0);
