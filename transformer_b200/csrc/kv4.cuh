@@ -720,6 +720,9 @@ constexpr __host__ __device__ int kv4_attn_smem() {
 // A page's bytes are contiguous: each comes by one bulk copy into the warp's
 // ring, kKv4Ahead steps ahead; a step takes P pages, so the running maximum
 // and the rescaling of o are paid once for 16 P positions.
+// One row of 32 heads over 8 of 128 dims on 131071 positions: 46 us with the join, 3.3
+// TB/s; 32 such rows on 1001 to 16384: 91 us, 3.5 TB/s.  Bound by instructions, 393 a
+// page of 2304 bytes, most of them turning codes to halves, at 64% of the issue slots.
 template <class T, int NH, int NB>
 __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
   constexpr int W = kKv4Warps, D = 64 * NH, COLS = 8 * NB, P = kv4_step_pages(NH), PB = kv4_page_bytes(D), SLOTS = kKv4Ahead + 1;
