@@ -1,0 +1,62 @@
+"""GPU: the 4-bit cache's operators at the ends of their ranges, against their
+definition in 64 bits (tests/kv4_ref.py)."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+import kv4_ref as R
+from transformer_b200.kv4 import check_status, kv4_append, kv4_attention, kv4_read, new_kv4_pool
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"bf16": torch.bfloat16, "f16": torch.float16}
+
+
+def f64(t):
+    return t.double().cpu().numpy()
+
+
+def i32(a, dev):
+    return torch.as_tensor(np.asarray(a), dtype=torch.int32).to(dev)
+
+
+def filled(k, v, cuda):
+    """A cache of one sequence that holds the rows k, v [length, n_kv, d]:
+    (pool, table, the held rows in 64 bits)."""
+    length, n_kv, d = k.shape
+    pages = (length + 15) // 16
+    pool = new_kv4_pool(pages, n_kv, d, cuda)
+    table = i32(np.random.default_rng(length).permutation(pages)[None], cuda)
+    at, zero = i32(np.arange(length), cuda), i32(np.zeros(length), cuda)
+    kv4_append(pool, *(torch.from_numpy(x.astype(np.float32)).to(cuda) for x in (k, v)), at, table, seq=zero)
+    return pool, table, *(f64(x) for x in kv4_read(pool, at, table, seq=zero, dtype=torch.float32))
+
+
+# a length, the rows that ask, heads a kv head: one token alone, with two blocks of
+# columns, and split over the positions; a prompt's chunk of one group of columns
+# and split over the positions
+SHAPES = [(50, 1, 4), (50, 3, 5), (4001, 1, 4), (130, 40, 2), (4100, 35, 3)]
+
+
+@pytest.mark.parametrize("length,rows,group", SHAPES)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("apart", [20, 27, 34])
+def test_queries_of_wide_range(cuda, length, rows, group, d, apart):
+    """bf16 query dims 2^apart below the row's largest count like the others:
+    the keys are as much larger there, so both halves of the dims make the score."""
+    rng = np.random.default_rng(length + d + apart)
+    n_kv, far = 2, 2.0 ** (apart / 2)
+    ratio = np.where(np.arange(d) % 32 < 16, far, 1 / far)  # (scales are per 16 dims)
+    k = rng.normal(size=(length, n_kv, d)) / ratio * np.minimum(1, 2000 / far)  # (held magnitudes reach 64512)
+    pool, table, hk, hv = filled(k, rng.normal(size=k.shape), cuda)
+    q = torch.from_numpy(rng.normal(size=(rows, n_kv * group, d)) * ratio * np.maximum(1, far / 2000))
+    q = q.to(torch.bfloat16).to(cuda)
+    start = None if rows == 1 else i32([0, rows], cuda)
+    out = kv4_attention(q, pool, i32([length], cuda), table, q_start=start)
+    want, mass, size = R.attention(f64(q), hk, hv, d ** -0.5)
+    bound = R.attention_bound(want, mass, size, length, d, 2.0 ** -8, np.abs(hv).max())
+    err = np.abs(f64(out) - want)
+    assert (err <= bound).all(), float((err / bound).max())

@@ -23,6 +23,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "b2d_ptx.cuh"
 #include "kv4.h"
 
@@ -246,8 +248,10 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float (&hi)[8], const flo
 }
 
 // Four pairs of halves of a code word: nibbles (i, i + 4) for i = 0 .. 3, each
-// times its scale.  1024 + u (bits 0-3 of a half's mantissa) less 1032, or
-// 1024 + 16 u (bits 4-7) over 16 less 72, is u - 8 exactly; so is the product.
+// times its scale.  (Bits put into the mantissa of a power of two make a float of
+// a small whole number, the common way around a conversion.)  1024 + u (bits 0-3
+// of a half's mantissa) less 1032, or 1024 + 16 u (bits 4-7) over 16 less 72, is
+// u - 8 exactly; so is the product.
 __device__ __forceinline__ void kv4_values(uint32_t w, uint32_t s, uint32_t (&v)[4]) {
   const uint32_t x = w >> 8;
   asm("{\n\t.reg .b32 a, b, c, d;\n\t"
@@ -265,6 +269,30 @@ __device__ __forceinline__ void kv4_values(uint32_t w, uint32_t s, uint32_t (&v)
       "mul.rn.f16x2 %3, d, %6;\n\t}"
       : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
       : "r"(w), "r"(x), "r"(s), "r"(0x64086408u), "r"(0x2C002C00u), "r"(0xD480D480u));
+}
+
+// A pair of scales for pairs of bf16 values, and -136 times it (17 times 8 times
+// at most 4 bits: 8 bits, exact).  A scale's 8 bits lie in a bf16's as they do in
+// a half's, with an exponent 112 less; below 2^-14 they are subnormal in both.
+struct Kv4ScaleBf {
+  uint32_t s, c;
+};
+__device__ __forceinline__ Kv4ScaleBf kv4_scales_bf(uint32_t w, uint32_t selector) {  // selector as in kv4_scales
+  Kv4ScaleBf k;
+  const uint32_t b = __byte_perm(w, 0u, selector) * 16u;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(k.s) : "r"(b), "r"(0x77807780u));    // 2^112
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(k.c) : "r"(k.s), "r"(0xC308C308u));  // -136
+  return k;
+}
+// kv4_values as bf16: 128 + u times the scale less 136 times it, exact in one step.
+__device__ __forceinline__ void kv4_values(uint32_t w, const Kv4ScaleBf& k, uint32_t (&v)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    asm("{\n\t.reg .b32 a;\n\t"
+        "lop3.b32 a, %1, 0x000F000F, 0x43004300, 0xEA;\n\t"
+        "fma.rn.bf16x2 %0, a, %2, %3;\n\t}"
+        : "=r"(v[i])
+        : "r"(w >> (4 * i)), "r"(k.s), "r"(k.c));
 }
 
 // ---- append ------------------------------------------------------------------------
@@ -509,19 +537,17 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const __grid_constant__ K
 }
 
 // ---- attention -----------------------------------------------------------------------
-// S^T = K Q^T and O^T = V^T P^T on m16n8k16 in half: the 16 positions of a page
+// S^T = K Q^T and O^T = V^T P^T on m16n8k16: the 16 positions of a page
 // are the rows of the first product and the reduction of the second, the query
 // columns (row of the sequence, head of the group) its 8 columns, so no
 // fragment of the cache is wasted on absent queries.
 //
 // Both operands of both products are exact but for the probabilities: held
-// values are halves, half queries are taken as they are, and bf16 queries (8
-// significant bits) become halves after each column is divided by the power of
-// two below its largest magnitude, which the softmax scale takes back; what
-// that loses of dims 2^28 times smaller than the largest is far below a
-// float32 sum's own rounding.  Probabilities keep 11 bits: they carry a factor
-// 2^15, so those down to 2^-29 of the row's largest are normal halves, and the
-// sum they are divided by carries it too.
+// values are exact in bf16 and in half, so S is formed in the queries' own type
+// (as halves under a power of two per column, bf16 queries lost what lies 2^17
+// below their row's largest, and a wave of 256 took 14.5 us, not 13.9) and O in half.  Probabilities keep 11 bits: they
+// carry a factor 2^15, so those down to 2^-29 of the row's largest are normal
+// halves, and the sum they are divided by carries it too.
 constexpr float kKv4POffset = 15.f;
 
 // Scale pair from two bytes of w: selector 0x4i4j puts bytes j, i into the halves.
@@ -546,9 +572,31 @@ __device__ __forceinline__ void mma_half_first(float (&d)[4], uint32_t a0, uint3
       : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
-// A column's query fragments: f[h][2 s], f[h][2 s + 1] for k-step s, dims (s, s + 4)
-// and (8 + s, 12 + s) of the lane's 16 at q + 64 h.  Returns the power of two the
-// column was divided by (the four lanes of a column agree on it).
+// The same on pairs of T, bf16 or half.
+template <class T>
+__device__ __forceinline__ void mma_scores(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                           uint32_t b0, uint32_t b1, bool first) {
+  if constexpr (std::is_same<T, __half>::value) {
+    if (first) mma_half_first(d, a0, a1, a2, a3, b0, b1);
+    else mma_half(d, a0, a1, a2, a3, b0, b1);
+  } else if (first) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%10, %10, %10, %10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+  } else {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  }
+}
+// A pair of scales for values of type T.
+template <class T>
+__device__ __forceinline__ auto kv4_scales_of(uint32_t w, uint32_t selector) {
+  if constexpr (std::is_same<T, __half>::value) return kv4_scales(w, selector);
+  else return kv4_scales_bf(w, selector);
+}
 template <class T>
 __device__ __forceinline__ void load16(const T* p, uint32_t (&w)[8], bool in, bool vec) {  // 16 elements of 2 bytes
   if (!in) {
@@ -564,8 +612,10 @@ __device__ __forceinline__ void load16(const T* p, uint32_t (&w)[8], bool in, bo
     for (int i = 0; i < 8; ++i) w[i] = b[2 * i] | (static_cast<uint32_t>(b[2 * i + 1]) << 16);
   }
 }
-template <int NH>
-__device__ __forceinline__ float kv4_query(const __half* q, bool in, bool vec, uint32_t (&f)[NH][8]) {
+// A column's query fragments: f[h][2 s], f[h][2 s + 1] for k-step s, dims (s, s + 4)
+// and (8 + s, 12 + s) of the lane's 16 at q + 64 h.
+template <int NH, class T>
+__device__ __forceinline__ void kv4_query(const T* q, bool in, bool vec, uint32_t (&f)[NH][8]) {
 #pragma unroll
   for (int h = 0; h < NH; ++h) {
     uint32_t w[8];
@@ -577,35 +627,6 @@ __device__ __forceinline__ float kv4_query(const __half* q, bool in, bool vec, u
       f[h][2 * s + 1] = __byte_perm(w[4 + (s >> 1)], w[6 + (s >> 1)], sel);
     }
   }
-  return 1.f;
-}
-template <int NH>
-__device__ __forceinline__ float kv4_query(const __nv_bfloat16* q, bool in, bool vec, uint32_t (&f)[NH][8]) {
-  uint32_t w[NH][8], top = 0;
-#pragma unroll
-  for (int h = 0; h < NH; ++h) {
-    load16(q + 64 * h, w[h], in, vec);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t x = w[h][i] & 0x7F807F80u;  // both exponents, the upper one leading
-      top = max(top, max(x, x << 16));
-    }
-  }
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2)) >> 23;
-  const int e = top == 0 ? 0 : min(static_cast<int>(top), 253) - 127;
-  const float down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-#pragma unroll
-  for (int h = 0; h < NH; ++h)
-#pragma unroll
-    for (int s = 0; s < 4; ++s)
-#pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t x = w[h][4 * k + (s >> 1)], y = w[h][4 * k + 2 + (s >> 1)];
-        f[h][2 * s + k] = s & 1 ? pack_half2(bf16_hi(x) * down, bf16_hi(y) * down)
-                                : pack_half2(bf16_lo(x) * down, bf16_lo(y) * down);
-      }
-  return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 }
 
 __device__ __forceinline__ float exp2_fast(float x) {  // 2^x (2 ulp), 0 at -infinity
@@ -803,7 +824,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
 
   // query fragments: column gid of each block, dims 64h + 16 tig .. in the codes' order
   uint32_t qf[NB][NH][8];
-  float up[NB][2];  // softmax scales of columns 2 tig, 2 tig + 1
+  const float up = a.scale_log2;
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb) {
     const int col = c0 + 8 * nb + gid;
@@ -811,9 +832,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
     const int row = in && tl.rows > 1 ? kv4_row(a, col) : 0, head = in ? col - row * a.group : 0;
     const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(tl.r0 + row) * a.q_row +
                  static_cast<int64_t>(tl.g * a.group + head) * a.q_head + 16 * tig;
-    const float scale = a.scale_log2 * kv4_query<NH>(q, in, aligned16(a.q, a.q_row, a.q_head, sizeof(T)), qf[nb]);
-    up[nb][0] = __shfl_sync(0xffffffffu, scale, 8 * tig);
-    up[nb][1] = __shfl_sync(0xffffffffu, scale, 8 * tig + 4);
+    kv4_query<NH>(q, in, aligned16(a.q, a.q_row, a.q_head, sizeof(T)), qf[nb]);
   }
   // columns 2 tig, 2 tig + 1 of each block: the positions they see
   int lim[NB][2];
@@ -855,7 +874,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
       for (int h = 0; h < NH; ++h) {
         const uint4 kc = reinterpret_cast<const uint4*>(page)[h * 32 + lane];
         const uint32_t kb = reinterpret_cast<const uint16_t*>(page + 8 * D)[h * 32 + lane];
-        const uint32_t s0 = kv4_scales(kb, 0x4040), s1 = kv4_scales(kb, 0x4141);
+        const auto s0 = kv4_scales_of<T>(kb, 0x4040), s1 = kv4_scales_of<T>(kb, 0x4141);
         uint32_t k0[4], k1[4], k2[4], k3[4];
         kv4_values(kc.x, s0, k0);
         kv4_values(kc.z, s1, k1);
@@ -864,10 +883,9 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
 #pragma unroll
         for (int s = 0; s < 4; ++s)
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            if (h == 0 && s == 0) mma_half_first(sc[p][nb], k0[s], k1[s], k2[s], k3[s], qf[nb][h][0], qf[nb][h][1]);
-            else mma_half(sc[p][nb], k0[s], k1[s], k2[s], k3[s], qf[nb][h][2 * s], qf[nb][h][2 * s + 1]);
-          }
+          for (int nb = 0; nb < NB; ++nb)
+            mma_scores<T>(sc[p][nb], k0[s], k1[s], k2[s], k3[s], qf[nb][h][2 * s], qf[nb][h][2 * s + 1],
+                          h == 0 && s == 0);
       }
     }
     // softmax of the step's positions: rows gid (c0, c1) and gid + 8 (c2, c3) of each page
@@ -897,14 +915,14 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
         const float mn = fmaxf(m[nb][e], mx), ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: all zero
-        al[e] = exp2_fast((m[nb][e] - ref) * up[nb][e]);
+        al[e] = exp2_fast((m[nb][e] - ref) * up);
         m[nb][e] = mn;
-        const float sub = fmaf(-ref, up[nb][e], kKv4POffset);
+        const float sub = fmaf(-ref, up, kKv4POffset);
         float sum = 0.f;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-          sc[p][nb][e] = exp2_fast(fmaf(sc[p][nb][e], up[nb][e], sub));
-          sc[p][nb][2 + e] = exp2_fast(fmaf(sc[p][nb][2 + e], up[nb][e], sub));
+          sc[p][nb][e] = exp2_fast(fmaf(sc[p][nb][e], up, sub));
+          sc[p][nb][2 + e] = exp2_fast(fmaf(sc[p][nb][2 + e], up, sub));
           sum += sc[p][nb][e] + sc[p][nb][2 + e];
         }
         l[nb][e] = fmaf(l[nb][e], al[e], sum);
@@ -1011,7 +1029,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
       const int col = 8 * nb + 2 * tig + e;
       if (c0 + col >= cols) continue;
       if (gid == 0) {
-        s_m[warp][col] = m[nb][e] * up[nb][e];
+        s_m[warp][col] = m[nb][e] * up;
         s_l[warp][col] = l[nb][e];
       }
 #pragma unroll

@@ -7,12 +7,12 @@
 //   S = Q K^T   M = 128 columns, N = 64 positions, K = d; Q and K in shared memory
 //   O += P V    M = 128 columns, N = d, K = 64 positions; P in tensor memory, V in
 //               shared memory
-// with the halves of kv4.cuh (held values, queries and scores exact, P with 11
-// bits and a factor 2^10).  Its warps have parts, which meet only on mbarriers (for
+// with the operands of kv4.cuh (held values and queries exact, S in the queries'
+// type, P with 11 bits and a factor 2^10).  Its warps have parts, which meet only on mbarriers (for
 // two groups):
 //   warps 0-7    softmax: thread r owns column r, lane r % 128 of its group's
 //                tensor memory
-//   warps 8-11   turn K's codes to halves, a page of each tile, straight into the
+//   warps 8-11   turn K's codes to values, a page of each tile, straight into the
 //                swizzled operand
 //   warps 12-15  V's
 //   warps 16-17  issue a group's products
@@ -43,7 +43,6 @@
 #pragma once
 
 #include <climits>
-#include <type_traits>
 
 #include "kv4.cuh"
 #include "tc_ptx.cuh"
@@ -221,30 +220,12 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
   const int col = c0 + tid, gr = warp >> 2;
   const bool in = warp < CODES && col < cols;
   const int row = in && tl.rows > 1 ? kv4_row(a, col) : 0, head = in ? col - row * a.group : 0;
-  float up = a.scale_log2;
+  const float up = a.scale_log2;
   if (warp < CODES) {
-    // halves, dims in the codes' order, to row tid of its group's Q
+    // dims in the codes' order, to row tid of its group's Q
     const T* q = static_cast<const T*>(a.q) + static_cast<int64_t>(tl.r0 + row) * a.q_row +
                  static_cast<int64_t>(tl.g * a.group + head) * a.q_head;
     const bool vec = aligned16(a.q, a.q_row, a.q_head, sizeof(T));
-    float down = 1.f;
-    if constexpr (sizeof(T) == 2 && !std::is_same<T, __half>::value) {
-      uint32_t top = 0;
-#pragma unroll
-      for (int b = 0; b < D / 16; ++b) {
-        uint32_t w[8];
-        load16(q + 16 * b, w, in, vec);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const uint32_t x = w[i] & 0x7F807F80u;
-          top = max(top, max(x, x << 16));
-        }
-      }
-      top >>= 23;
-      const int e = top == 0 ? 0 : min(static_cast<int>(top), 253) - 127;
-      down = __uint_as_float(static_cast<uint32_t>(127 - e) << 23);
-      up *= __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
-    }
 #pragma unroll
     for (int b = 0; b < D / 16; ++b) {
       uint32_t w[8], f[8];
@@ -254,11 +235,7 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
 #pragma unroll
         for (int k = 0; k < 2; ++k) {  // pair s of block k: dims (8k + s, 8k + s + 4)
           const uint32_t x = w[4 * k + (s >> 1)], y = w[4 * k + 2 + (s >> 1)];
-          if constexpr (std::is_same<T, __half>::value)
-            f[4 * k + s] = __byte_perm(x, y, s & 1 ? 0x7632 : 0x5410);
-          else
-            f[4 * k + s] = s & 1 ? pack_half2(bf16_hi(x) * down, bf16_hi(y) * down)
-                                 : pack_half2(bf16_lo(x) * down, bf16_lo(y) * down);
+          f[4 * k + s] = __byte_perm(x, y, s & 1 ? 0x7632 : 0x5410);
         }
       uint8_t* dst = sq + (gr * NH + (b >> 2)) * 16384 + (tid & 127) * 128;
       const int c = (b & 3) * 2;
@@ -294,7 +271,8 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
       for (int k = 0; k < D / 16; ++k) {
         const uint64_t qd = sdesc_kmajor_sw128(q0 + (k >> 2) * 16384 + (k & 3) * 32);
         const uint64_t kd = sdesc_kmajor_sw128(k0 + (i & 1) * K_BUF + (k >> 2) * 8192 + (k & 3) * 32);
-        if (leader) tc_mma_bf16(t_s + 64 * (i & 1), qd, kd, idesc_f16_f32(128, 64), k > 0);
+        constexpr uint32_t idesc = std::is_same<T, __half>::value ? idesc_f16_f32(128, 64) : idesc_bf16_f32(128, 64);
+        if (leader) tc_mma_bf16(t_s + 64 * (i & 1), qd, kd, idesc, k > 0);  // (the type is the descriptor's)
       }
       if (leader) tc_commit(&s_bar[kSDone + g][i & 1]);
       return true;
@@ -312,7 +290,7 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
       }
       if (leader) tc_commit(&s_bar[kODone + g][i & 1]);
     }
-  } else if (warp >= CODES) {  // ---- codes to halves ----
+  } else if (warp >= CODES) {  // ---- codes to values ----
     const int32_t* table = a.c.table + tl.seq * a.c.table_ld;
     const uint8_t* pool = a.c.pool + static_cast<int64_t>(tl.g) * PB;
     const int64_t block_bytes = static_cast<int64_t>(a.c.n_kv) * PB;
@@ -372,7 +350,7 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
               if (i >= 2 && !wait(kSDone + g, i - 2)) return false;
 #pragma unroll
             for (int h = 0; h < NH; ++h) {
-              const uint32_t s0 = kv4_scales(kf.scale[h], 0x4040), s1 = kv4_scales(kf.scale[h], 0x4141);
+              const auto s0 = kv4_scales_of<T>(kf.scale[h], 0x4040), s1 = kv4_scales_of<T>(kf.scale[h], 0x4141);
               uint32_t v[4];
               uint8_t* d0 = k_to + (i & 1) * K_BUF + h * 8192;
               uint8_t* d1 = d0 + 2 * 128;
