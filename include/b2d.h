@@ -442,8 +442,8 @@ typedef struct {
  * Causal attention: a sequence's n rows are its last n positions, row j of
  * them sees positions 0 .. len - n + j.  A row that sees nothing is zero.
  * Sequence i uses table row i; head h reads kv head h / (n_heads /
- * n_kv_heads).  Products and sums in float32, probabilities held in 11
- * bits.  Results do not depend on the run: every sum has a fixed order.
+ * n_kv_heads).  Products and sums in float32 (as are scores before their
+ * scale: 3.4e38 bounds them), probabilities held in 11 bits.  Results do not depend on the run: every sum has a fixed order.
  * `scratch_dev` (16-byte aligned) holds the partial results of split
  * sequences: b2d_kv4_attention_scratch says how many bytes, 0 for none.  Calls
  * that may overlap need scratch of their own.

@@ -60,3 +60,26 @@ def test_queries_of_wide_range(cuda, length, rows, group, d, apart):
     bound = R.attention_bound(want, mass, size, length, d, 2.0 ** -8, np.abs(hv).max())
     err = np.abs(f64(out) - want)
     assert (err <= bound).all(), float((err / bound).max())
+
+
+@pytest.mark.parametrize("length,rows,group", SHAPES)
+@pytest.mark.parametrize("dtype,d", [("bf16", 64), ("f16", 64), ("bf16", 128), ("f16", 128)])
+@pytest.mark.parametrize("top", [1.0, 2.0 ** 5, 2.0 ** 11])
+def test_scores_of_any_size(cuda, length, rows, group, dtype, d, top):
+    """Scores to 2^30: finite, and shares of the rows that reach the largest.
+    Keys are 0 or the cache's largest value, queries small whole numbers times
+    `top`, so that every score is exact in 32 bits: those that are not the
+    row's largest are too far below it to count."""
+    rng = np.random.default_rng(length + d + int(top))
+    n_kv, held = 2, 64512.0
+    k = held * rng.integers(-1, 2, size=(7, n_kv, d))[rng.integers(0, 7, length)]  # seven rows, each many times
+    pool, table, hk, hv = filled(k, rng.normal(size=k.shape), cuda)
+    assert np.array_equal(hk, k)
+    q = top * rng.integers(-15, 16, size=(rows, n_kv * group, d))
+    out = kv4_attention(torch.from_numpy(q).to(TYPES[dtype]).to(cuda), pool, i32([length], cuda), table,
+                        q_start=None if rows == 1 else i32([0, rows], cuda))
+    want, mass, _ = R.attention(q, hk, hv, d ** -0.5)
+    # (no score is off, and none that counts has an argument other than 0)
+    bound = R.attention_bound(want, mass, 0.0, length, d, torch.finfo(TYPES[dtype]).eps / 2, np.abs(hv).max())
+    err = np.abs(f64(out) - want)
+    assert (err <= bound).all(), float(np.nanmax(err / bound))

@@ -548,6 +548,11 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const __grid_constant__ K
 // below their row's largest, and a wave of 256 took 14.5 us, not 13.9) and O in half.  Probabilities keep 11 bits: they
 // carry a factor 2^15, so those down to 2^-29 of the row's largest are normal
 // halves, and the sum they are divided by carries it too.
+//
+// An exponent is the difference of two scores first, then scaled: scaled scores
+// apart, each rounded at its own size, would be off by more than the factor's room
+// from 2^25 on.  (An instruction more a score: 45.9 us, not 45.6, on 131071
+// positions; prompts' chunks 151, not 149.)
 constexpr float kKv4POffset = 15.f;
 
 // Scale pair from two bytes of w: selector 0x4i4j puts bytes j, i into the halves.
@@ -688,7 +693,8 @@ __device__ __forceinline__ int kv4_tile_pages(const Kv4AttnArgs& a, const Kv4Til
   return (kv4_limit(a, t, last) + kKv4Page - 1) / kKv4Page;
 }
 
-// A split's share of a column: d floats of o, then its maximum and sum.
+// A split's share of a column: d floats of o, then its maximum (of the scores
+// before their scale) and sum.
 __device__ __forceinline__ float* kv4_part(const Kv4AttnArgs& a, int seq, int g, int tile, int split, int col, int d) {
   const int64_t unit = (static_cast<int64_t>(seq) * a.c.n_kv + g) * a.tiles + tile;
   return a.part + ((unit * a.splits + split) * a.tile_cols + col) * (d + 4);
@@ -917,12 +923,11 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
         const float mn = fmaxf(m[nb][e], mx), ref = mn == -INFINITY ? 0.f : mn;  // nothing seen yet: all zero
         al[e] = exp2_fast((m[nb][e] - ref) * up);
         m[nb][e] = mn;
-        const float sub = fmaf(-ref, up, kKv4POffset);
         float sum = 0.f;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-          sc[p][nb][e] = exp2_fast(fmaf(sc[p][nb][e], up, sub));
-          sc[p][nb][2 + e] = exp2_fast(fmaf(sc[p][nb][2 + e], up, sub));
+          sc[p][nb][e] = exp2_fast(fmaf(sc[p][nb][e] - ref, up, kKv4POffset));
+          sc[p][nb][2 + e] = exp2_fast(fmaf(sc[p][nb][2 + e] - ref, up, kKv4POffset));
           sum += sc[p][nb][e] + sc[p][nb][2 + e];
         }
         l[nb][e] = fmaf(l[nb][e], al[e], sum);
@@ -1029,7 +1034,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
       const int col = 8 * nb + 2 * tig + e;
       if (c0 + col >= cols) continue;
       if (gid == 0) {
-        s_m[warp][col] = m[nb][e] * up;
+        s_m[warp][col] = m[nb][e];
         s_l[warp][col] = l[nb][e];
       }
 #pragma unroll
@@ -1051,7 +1056,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
     const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float f = exp2_fast(s_m[w][col] - ref);
+      const float f = exp2_fast((s_m[w][col] - ref) * up);
       L = fmaf(f, s_l[w][col], L);
       const float4 x = *reinterpret_cast<const float4*>(&s_o[w][col][d0]), y = *reinterpret_cast<const float4*>(&s_o[w][col][d0 + 4]);
       r[0] = fmaf(f, x.x, r[0]); r[1] = fmaf(f, x.y, r[1]); r[2] = fmaf(f, x.z, r[2]); r[3] = fmaf(f, x.w, r[3]);
@@ -1097,7 +1102,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ K
     }
 #pragma unroll
     for (int i = 0; i < DEEP; ++i) {
-      const float f = exp2_fast(ml[i].x - ref);
+      const float f = exp2_fast((ml[i].x - ref) * a.scale_log2);
       L = fmaf(f, ml[i].y, L);
 #pragma unroll
       for (int h = 0; h < NH; ++h) {

@@ -464,9 +464,8 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
           }
         }
       }
-      const float sub = fmaf(m == -INFINITY ? 0.f : -m, up, kKv4PromptOffset);
-      const uint64_t up2 = pair_of(__float_as_uint(up), __float_as_uint(up));
-      const uint64_t sub2 = pair_of(__float_as_uint(sub), __float_as_uint(sub));
+      auto twice = [](float x) { return pair_of(__float_as_uint(x), __float_as_uint(x)); };
+      const uint64_t up2 = twice(up), offset2 = twice(kKv4PromptOffset), minus2 = twice(m == -INFINITY ? 0.f : -m);
       uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int c = 0; c < 64; c += 32) {
@@ -474,7 +473,7 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
         uint32_t p[16];
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
-          const float2 e = floats_of(fma2(pair_of(s[2 * k], s[2 * k + 1]), up2, sub2));
+          const float2 e = floats_of(fma2(add2(pair_of(s[2 * k], s[2 * k + 1]), minus2), up2, offset2));
           const float x = exp2_fast(e.x), y = exp2_fast(e.y);
           sum[k & 1] = add2(sum[k & 1], pair_of(__float_as_uint(x), __float_as_uint(y)));
           p[k] = pack_half2(x, y);
@@ -525,7 +524,7 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
       }
     }
     if (in && a.splits > 1)
-      *reinterpret_cast<float2*>(kv4_part(a, tl.seq, tl.g, tl.tile, tl.split, tid, D) + D) = make_float2(m * up, l);
+      *reinterpret_cast<float2*>(kv4_part(a, tl.seq, tl.g, tl.tile, tl.split, tid, D) + D) = make_float2(m, l);
   }
   if (s_fail && tid == 0) {  // what was issued may still be running: a bounded wait for it
     kv4_error(a.c.status, kKv4Timeout);
