@@ -443,7 +443,11 @@ typedef struct {
  * them sees positions 0 .. len - n + j.  A row that sees nothing is zero.
  * Sequence i uses table row i; head h reads kv head h / (n_heads /
  * n_kv_heads).  Products and sums in float32 (as are scores before their
- * scale: 3.4e38 bounds them), probabilities held in 11 bits.  Results do not depend on the run: every sum has a fixed order.
+ * scale: 3.4e38 bounds them), probabilities held in 11 bits.  Results do not
+ * depend on the run: every sum has a fixed order.
+ * What sets the status: a sequence longer than max_len counts as an empty one
+ * (zero rows), rows out of range are not written, and a row that sees a
+ * position of a block that the table does not name is zero.
  * `scratch_dev` (16-byte aligned) holds the partial results of split
  * sequences: b2d_kv4_attention_scratch says how many bytes, 0 for none.  Calls
  * that may overlap need scratch of their own.

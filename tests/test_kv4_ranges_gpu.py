@@ -83,3 +83,44 @@ def test_scores_of_any_size(cuda, length, rows, group, dtype, d, top):
     bound = R.attention_bound(want, mass, 0.0, length, d, torch.finfo(TYPES[dtype]).eps / 2, np.abs(hv).max())
     err = np.abs(f64(out) - want)
     assert (err <= bound).all(), float(np.nanmax(err / bound))
+
+
+@pytest.mark.parametrize("dtype,heads,n_kv,d,lens,rows", [
+    ("bf16", 16, 4, 64, [1, 17, 64, 130, 333, 48], None), ("f16", 10, 2, 128, [70, 16, 5000], None),
+    ("bf16", 8, 8, 128, [9001], None), ("bf16", 8, 2, 64, [130, 77], [40, 77]), ("f16", 32, 8, 128, [260, 70], [90, 70]),
+    ("f16", 8, 2, 128, [5003, 4100], [70, 33]), ("bf16", 16, 4, 64, [700, 400, 720], [600, 350, 600])])
+def test_blocks_that_the_table_does_not_name(cuda, dtype, heads, n_kv, d, lens, rows):
+    """A row that sees a position of one is zero, others (before it) as ever, and
+    the status is set.  One token alone, split, with two blocks of columns; chunks
+    of one and two groups of columns, and split."""
+    rng = np.random.default_rng(sum(lens) + d)
+    bps, counts = (max(lens) + 15) // 16, rows or [1] * len(lens)
+    blocks = len(lens) * bps
+    pool, table = new_kv4_pool(blocks, n_kv, d, cuda), rng.permutation(blocks).reshape(len(lens), bps)
+    held = []
+    for i, n in enumerate(lens):
+        k, v = (torch.from_numpy(rng.normal(size=(n, n_kv, d)).astype(np.float32)).to(cuda) for _ in range(2))
+        at, seq = i32(np.arange(n), cuda), i32(np.full(n, i), cuda)
+        kv4_append(pool, k, v, at, i32(table, cuda), seq=seq)
+        held.append([f64(x) for x in kv4_read(pool, at, i32(table, cuda), seq=seq, dtype=torch.float32)])
+    lost = np.zeros(table.shape, bool)
+    lost[0, (lens[0] - counts[0] // 2 - 1) // 16] = True  # seen by a token, by half of a chunk's rows
+    lost[-1, rng.integers(0, (lens[-1] + 15) // 16, 2)] = True
+    bad = np.where(lost, rng.choice([-1, blocks, 2 ** 31 - 1, -2 ** 31], table.shape), table)
+    q = torch.from_numpy(rng.normal(size=(sum(counts), heads, d))).to(TYPES[dtype]).to(cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    start = None if rows is None else i32(np.cumsum([0, *rows]), cuda)
+    out = kv4_attention(q, pool, i32(lens, cuda), i32(bad, cuda), q_start=start, status=status)
+    assert int(status.item()) == 0x203
+    at, some = 0, False
+    for i, (n, c, (k, v)) in enumerate(zip(lens, counts, held)):
+        want, mass, size = R.attention(f64(q)[at:at + c], k, v, d ** -0.5)
+        bound = R.attention_bound(want, mass, size, n, d, torch.finfo(TYPES[dtype]).eps / 2, np.abs(v).max())
+        first = np.flatnonzero(lost[i, :(n + 15) // 16])
+        zero = np.arange(n - c, n) >= (16 * first[0] if first.size else n)
+        want[zero], bound[zero] = 0.0, 0.0
+        err = np.abs(f64(out)[at:at + c] - want)
+        assert (err <= bound).all(), i
+        some = some or (zero.any() and not zero.all())
+        at += c
+    assert some or rows is None  # (rows on both sides of a lost block)

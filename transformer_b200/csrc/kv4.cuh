@@ -23,6 +23,7 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <climits>
 #include <type_traits>
 
 #include "b2d_ptx.cuh"
@@ -53,6 +54,8 @@ __device__ __forceinline__ void kv4_error(uint32_t* status, uint32_t code) {
 }
 constexpr uint32_t kKv4BadPos = 0x202u, kKv4BadTable = 0x203u, kKv4Timeout = 0x10Du;
 
+// Whether the pool has the block that a table's entry names.
+__device__ __forceinline__ bool kv4_named(const Kv4Cache& c, int blk) { return blk >= 0 && blk < c.num_blocks; }
 // The page of position `pos` of the sequence with table row `sid`, or null
 // (status set) when the table does not name one.
 __device__ __forceinline__ uint8_t* kv4_page(const Kv4Cache& c, int sid, int pos, int g) {
@@ -62,7 +65,7 @@ __device__ __forceinline__ uint8_t* kv4_page(const Kv4Cache& c, int sid, int pos
     return nullptr;
   }
   const int blk = __ldg(c.table + sid * c.table_ld + pg);
-  if (blk < 0 || blk >= c.num_blocks) {
+  if (!kv4_named(c, blk)) {
     kv4_error(c.status, kKv4BadTable);
     return nullptr;
   }
@@ -693,6 +696,13 @@ __device__ __forceinline__ int kv4_tile_pages(const Kv4AttnArgs& a, const Kv4Til
   return (kv4_limit(a, t, last) + kKv4Page - 1) / kKv4Page;
 }
 
+// A row that sees a position of a block that the table does not name is zero: a
+// share of it without those positions would look like an answer.  Its share of a
+// column has an infinite maximum, next to which no other share counts, and a sum
+// and o of zero (as an infinite score would not: its sum is NaN).
+__device__ __forceinline__ float kv4_share(float m, float top, float scale_log2) {  // what a share counts for, 0 .. 1
+  return m == top ? 1.f : exp2_fast((m - top) * scale_log2);
+}
 // A split's share of a column: d floats of o, then its maximum (of the scores
 // before their scale) and sum.
 __device__ __forceinline__ float* kv4_part(const Kv4AttnArgs& a, int seq, int g, int tile, int split, int col, int d) {
@@ -788,13 +798,15 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
     return lane < P && k < n_mine ? __ldg(table + lo + warp + W * k) : -1;
   };
   int fill = 0;  // the slot that the next step's copies fill
+  int lost = INT_MAX;  // the warp's first position whose block the table does not name
   auto issue = [&](int step, int id) {
     if (step >= steps) return;
     const int slot = fill, n = min(P, n_mine - step * P);
-    const bool good = id >= 0 && id < a.c.num_blocks;
+    const bool good = kv4_named(a.c, id);
     const uint32_t in = __ballot_sync(0xffffffffu, lane < n && good);
     uint8_t* dst = ring + slot * P * PB;
-    if (__popc(in) != n) {  // a page that the table does not name counts as zeros
+    if (__popc(in) != n) {  // a page that the table does not name is read as zeros
+      lost = min(lost, (lo + warp + W * (step * P + __ffs(~in) - 1)) * kKv4Page);
       for (int p = 0; p < n; ++p)
         if (!((in >> p) & 1u))
           for (int i = lane * 16; i < PB; i += 512) *reinterpret_cast<uint4*>(dst + p * PB + i) = make_uint4(0, 0, 0, 0);
@@ -1005,6 +1017,18 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
       l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 8);
       l[nb][e] += __shfl_xor_sync(0xffffffffu, l[nb][e], 16);
     }
+  if (lost != INT_MAX) {
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        if (lost < lim[nb][e]) {
+          m[nb][e] = INFINITY;
+          l[nb][e] = 0.f;
+#pragma unroll
+          for (int j = 0; j < 4 * NH; ++j) o[nb][j][e] = o[nb][j][2 + e] = 0.f;
+        }
+  }
   const bool ovec = aligned16(a.out, a.o_row, a.o_head, sizeof(T));
   // 8 dims from d0 of column c (of the sequence): final, or this split's share
   auto put = [&](int c, int d0, float (&r)[8], float M, float L) {
@@ -1056,7 +1080,7 @@ __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_c
     const float ref = M == -INFINITY ? 0.f : M;
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float f = exp2_fast((s_m[w][col] - ref) * up);
+      const float f = kv4_share(s_m[w][col], ref, up);
       L = fmaf(f, s_l[w][col], L);
       const float4 x = *reinterpret_cast<const float4*>(&s_o[w][col][d0]), y = *reinterpret_cast<const float4*>(&s_o[w][col][d0 + 4]);
       r[0] = fmaf(f, x.x, r[0]); r[1] = fmaf(f, x.y, r[1]); r[2] = fmaf(f, x.z, r[2]); r[3] = fmaf(f, x.w, r[3]);
@@ -1102,7 +1126,7 @@ __global__ void __launch_bounds__(128) kv4_join_kernel(const __grid_constant__ K
     }
 #pragma unroll
     for (int i = 0; i < DEEP; ++i) {
-      const float f = exp2_fast((ml[i].x - ref) * a.scale_log2);
+      const float f = kv4_share(ml[i].x, ref, a.scale_log2);
       L = fmaf(f, ml[i].y, L);
 #pragma unroll
       for (int h = 0; h < NH; ++h) {

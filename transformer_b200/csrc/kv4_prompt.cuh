@@ -183,6 +183,7 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
   __shared__ uint64_t s_bar[kBars][2];
   __shared__ uint32_t s_tmem;
   __shared__ volatile uint32_t s_fail;
+  __shared__ int s_lost;  // the first page that the table does not name
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, gid = lane >> 2, tig = lane & 3;
   uint8_t* sq = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(kv4_prompt_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* sk = sq + NG * NH * 128 * 128;  // Q [NG][NH][128 rows][128 B], K [2][NH][64 rows][128 B]
@@ -205,6 +206,7 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
     for (int i = 0; i < 2 * kBars; ++i) mbar_init(&s_bar[i >> 1][i & 1], i < 2 * kSDone ? 4 : 1);  // 4 warps, or a commit
     fence_mbar_init();
     s_fail = 0u;
+    s_lost = INT_MAX;
   }
   const int c0 = tl.tile * NG * kKv4PromptCols, cols = tl.cols(a), tiles = (hi - lo + PAGES - 1) / PAGES;
   // Bounded wait for a barrier's phase of tile i; one that runs out marks the
@@ -302,8 +304,11 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
     };
     // null: zeros (past the split, or not named by the table)
     auto page_at = [&](int i, int blk) -> const uint8_t* {
-      if (blk >= 0 && blk < a.c.num_blocks) return pool + blk * block_bytes;
-      if (lane == 0 && lo + i * PAGES + mine < hi) kv4_error(a.c.status, kKv4BadTable);
+      if (kv4_named(a.c, blk)) return pool + blk * block_bytes;
+      if (lane == 0 && lo + i * PAGES + mine < hi) {
+        atomicMin(&s_lost, lo + i * PAGES + mine);  // (before the tile's K: softmax threads look at their end)
+        kv4_error(a.c.status, kKv4BadTable);
+      }
       return nullptr;
     };
     // Tile i, whose page is in f; f takes tile i + 2's, so that a load has a tile's
@@ -489,6 +494,12 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
     }
     if (tiles > 0) wait(kODone + gr, tiles - 1);
     tc_fence_after();
+    // (all of the tiles' pages have been looked up, and s_lost with them)
+    const bool none = s_lost < INT_MAX && s_lost * kKv4Page < lim;
+    if (none) {
+      m = INFINITY;
+      l = 0.f;
+    }
 
     // ---- the column's result ----
     const bool ovec = aligned16(a.out, a.o_row, a.o_head, sizeof(T));
@@ -518,6 +529,10 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
                  r, ovec);
         } else {
           float* dst = kv4_part(a, tl.seq, tl.g, tl.tile, tl.split, tid, D) + 64 * h + 8 * g;
+          if (none) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) r[k] = 0.f;
+          }
           *reinterpret_cast<float4*>(dst) = make_float4(r[0], r[1], r[2], r[3]);
           *reinterpret_cast<float4*>(dst + 4) = make_float4(r[4], r[5], r[6], r[7]);
         }
