@@ -124,3 +124,35 @@ def test_blocks_that_the_table_does_not_name(cuda, dtype, heads, n_kv, d, lens, 
         some = some or (zero.any() and not zero.all())
         at += c
     assert some or rows is None  # (rows on both sides of a lost block)
+
+
+@pytest.mark.parametrize("n", [7, 600])  # (a block per batch of heads, a warp a row)
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_append_skips_a_row_past_the_table_with_its_query(cuda, n, dtype):
+    """A position past the table's row, a block that the pool does not have and a
+    row that the table does not have: neither the pool nor q_out is written, in
+    place either; the other rows are as without them."""
+    t = TYPES.get(dtype, torch.float32)
+    heads, n_kv, d, bps = 5, 2, 64, 3
+    gen = torch.Generator().manual_seed(n)
+    q, k, v = (torch.randn(n, h, d, generator=gen).to(t).to(cuda) for h in (heads, n_kv, n_kv))
+    ang = torch.randn(200, d // 2, generator=gen)
+    kw = dict(cos=ang.cos().to(cuda), sin=ang.sin().to(cuda))
+    table = np.arange(n * bps).reshape(n, bps)
+    pos, seq = np.arange(n) % 48, np.arange(n)
+    bad = np.array([1, 3, 4, n - 1])
+    pos[1], seq[4] = 16 * bps + 5, n
+    table[3, pos[3] // 16], table[n - 1, pos[n - 1] // 16] = n * bps, -1
+    good = torch.ones(n, dtype=torch.bool, device=cuda)
+    good[torch.from_numpy(bad).to(cuda)] = False
+    want_pool, pool = (new_kv4_pool(n * bps, n_kv, d, cuda) for _ in range(2))
+    at, rows, table = i32(pos, cuda), i32(seq, cuda), i32(table, cuda)
+    want = kv4_append(want_pool, k[good], v[good], at[good], table, seq=rows[good], q=q[good], **kw)
+    for inplace in (False, True):
+        pool.zero_()
+        status = torch.zeros(1, dtype=torch.int32, device=cuda)
+        src = q.clone()
+        out = src if inplace else torch.full_like(q, 9.0)
+        kv4_append(pool, k, v, at, table, seq=rows, q=src, q_out=out, status=status, **kw)
+        assert int(status.item()) == 0x203 and torch.equal(pool, want_pool) and torch.equal(out[good], want)
+        assert torch.equal(out[~good], q[~good] if inplace else torch.full_like(q[~good], 9.0))

@@ -398,6 +398,8 @@ __global__ void __launch_bounds__(kKv4AppendThreads, 6) kv4_append_kernel(
     if (threadIdx.x == 0) kv4_error(a.c.status, kKv4BadPos);
     return;
   }
+  uint8_t* page = kv4_page(a.c, sid, pos, slice);
+  if (page == nullptr) return;  // (its query is skipped too)
   float c[8], s[8];
   if (turns) kv4_angles<ROPE>(a, pos, i0, c, s);
 
@@ -435,8 +437,6 @@ __global__ void __launch_bounds__(kKv4AppendThreads, 6) kv4_append_kernel(
     }
   }
   if (!do_k && !do_v) return;
-  uint8_t* page = kv4_page(a.c, sid, pos, slice);
-  if (page == nullptr) return;
   const int r = pos % kKv4Page, page_step = slices * kv4_page_bytes(a.c.d);
   if (do_k) {
     const int code_at = kv4_k_code(oct >> 1, r) + 4 * (oct & 1), scale_at = kv4_k_scale(a.c.d, oct >> 1, r);
