@@ -210,9 +210,10 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
   }
   const int c0 = tl.tile * NG * kKv4PromptCols, cols = tl.cols(a), tiles = (hi - lo + PAGES - 1) / PAGES;
   // Bounded wait for a barrier's phase of tile i; one that runs out marks the
-  // CTA, whose parts then leave their loops.
+  // CTA, whose parts then leave their loops, a warp's lanes together (the votes:
+  // 151 us, not 148, on the 4 chunks).
   auto wait = [&](int which, int i) {
-    if (kv4_wait(&s_bar[which][i & 1], static_cast<uint32_t>(i >> 1) & 1u)) return true;
+    if (__all_sync(0xffffffffu, kv4_wait(&s_bar[which][i & 1], static_cast<uint32_t>(i >> 1) & 1u))) return true;
     s_fail = 1u;
     return false;
   };
@@ -262,7 +263,7 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
     const bool leader = elect_one();
     const uint32_t q0 = smem_addr(sq) + g * NH * 16384, k0 = smem_addr(sk), v0 = smem_addr(sv);
     auto poll = [&](int which, int i) {
-      if (kv4_poll(&s_bar[which][i & 1], static_cast<uint32_t>(i >> 1) & 1u)) return true;
+      if (__all_sync(0xffffffffu, kv4_poll(&s_bar[which][i & 1], static_cast<uint32_t>(i >> 1) & 1u))) return true;
       s_fail = 1u;
       return false;
     };
@@ -541,15 +542,15 @@ __global__ void __launch_bounds__(kv4_prompt_threads<NG>(), 1) kv4_prompt_kernel
     if (in && a.splits > 1)
       *reinterpret_cast<float2*>(kv4_part(a, tl.seq, tl.g, tl.tile, tl.split, tid, D) + D) = make_float2(m, l);
   }
-  if (s_fail && tid == 0) {  // what was issued may still be running: a bounded wait for it
-    kv4_error(a.c.status, kKv4Timeout);
-    const uint64_t t0 = globaltimer_ns();
-    while (globaltimer_ns() - t0 < 200000000ull) {
-    }
-  }
   tc_fence_before();
-  __syncthreads();
-  if (warp == ISSUE) tmem_dealloc(s_tmem, NG * kKv4PromptTmem);
+  __syncthreads();  // (all parts have left their loops: a wait that ran out has set s_fail)
+  if (warp == ISSUE) {
+    if (s_fail) {  // what was issued may still be running: a bounded wait for it (0.2 s) before its memory goes
+      if (lane == 0) kv4_error(a.c.status, kKv4Timeout);
+      for (uint32_t i = 0; i < kKv4Tries; ++i) __nanosleep(1000);
+    }
+    tmem_dealloc(s_tmem, NG * kKv4PromptTmem);
+  }
 }
 
 }  // namespace b2d
