@@ -205,8 +205,9 @@ class ContinuousBatcher:
     def submit(self, prompt, max_tokens: int, temperature: float = 0.0, top_p: float = 1.0,
                rep_penalty: float = 1.0, seed: int | None = None, presence: float = 0.0, frequency: float = 0.0,
                logit_bias: dict | None = None, allowed=None) -> int:
-        """Queues a request; returns its id.  ``presence`` and ``frequency`` are
-        subtracted from the logits of tokens it has generated, once and times
+        """Queues a request; returns its id.  In this order: logits of tokens it
+        has generated are divided (those above 0) or multiplied by ``rep_penalty``;
+        ``presence`` and ``frequency`` are subtracted from them, once and times
         their count; ``logit_bias`` {token: value} is added; ``allowed`` are the
         only token ids it may draw, or a function of the list of its generated
         tokens that gives them (none: the request ends; so it does when the
@@ -655,7 +656,8 @@ class ContinuousBatcher:
         groups: dict = {}
         for i, r in enumerate(rows):
             if r is not None and not r.greedy:
-                groups.setdefault((r.temperature, r.top_p, r.rep_penalty), []).append(i)
+                # (the repetition penalty comes first: with rules it has been applied with them)
+                groups.setdefault((r.temperature, r.top_p, 1.0 if r.rules else r.rep_penalty), []).append(i)
         greedy_rows = [i for i, r in enumerate(rows) if r is not None and r.greedy]
         if greedy_rows:
             out[greedy_rows] = self._fetch(greedy_src, batch)[greedy_rows]
@@ -688,8 +690,9 @@ class ContinuousBatcher:
         return out
 
     def _apply_rules(self, logits: torch.Tensor, rows) -> set:
-        """The rules of the requests ``rows`` on their rows of ``logits``, in
-        place, in one ``adjust_logits`` call; returns the rows that allow no token."""
+        """The rules of the requests ``rows`` on their rows of ``logits``, and
+        their repetition penalties, in the order of ``adjust_logits``, in place;
+        returns the rows that allow no token."""
         ended = set()
         if not any(r is not None and r.rules for r in rows):
             return ended
@@ -699,14 +702,15 @@ class ContinuousBatcher:
         masked = any(r is not None and r.allowed is not None for r in rows)
         hist_cap = max([len(r.out) for r in rows if r is not None and r.rules] + [1])
         hist, ints = np.zeros((n, hist_cap), np.int32), np.zeros((2, n), np.int32)  # lengths of history, biases
-        penalty = np.zeros((2, n), np.float32)  # presence, frequency
+        penalty = np.zeros((3, n), np.float32)  # presence, frequency, repetition
+        penalty[2] = 1.0
         bias_ids, bias = np.zeros((n, n_bias), np.int32), np.zeros((n, n_bias), np.float32)
         allow = np.full((n, 32 * words), 1, np.uint8) if masked else None
         for i, r in enumerate(rows):
             if r is None or not r.rules:
                 continue
             hist[i, :len(r.out)], ints[0, i] = r.out, len(r.out)
-            penalty[:, i] = r.presence, r.frequency
+            penalty[:, i] = r.presence, r.frequency, r.rep_penalty
             if r.logit_bias:
                 k = ints[1, i] = len(r.logit_bias)
                 bias_ids[i, :k], bias[i, :k] = list(r.logit_bias), list(r.logit_bias.values())
@@ -726,7 +730,8 @@ class ContinuousBatcher:
             return torch.from_numpy(np.ascontiguousarray(a)).to(self.eng.device)
 
         lens = put(ints)
-        kw = dict(history=put(hist), hist_len=lens[0], presence=put(penalty[0]), frequency=put(penalty[1]))
+        values = put(penalty)
+        kw = dict(history=put(hist), hist_len=lens[0], presence=values[0], frequency=values[1], rep_penalty=values[2])
         if n_bias:
             kw.update(bias_ids=put(bias_ids), bias_values=put(bias), bias_len=lens[1])
         if masked:
