@@ -96,3 +96,15 @@ def test_rows_with_and_without_rules(monkeypatch):
             want.append(int(x.argmax()))
         argmax = torch.from_numpy(lg.argmax(-1).astype(np.int32))
         assert cb._sample_rows(torch.from_numpy(lg), rows, argmax).tolist() == want
+
+
+@pytest.mark.parametrize("kw", [dict(presence=1e300), dict(frequency=-1e39), dict(logit_bias={1: 0.5, 3: 3.5e38}),
+                                dict(logit_bias={0: -1e200}), dict(presence=2.0 ** 128)])
+def test_numbers_that_float32_does_not_hold_are_refused(kw):
+    """They would be infinite where they act."""
+    cb = ContinuousBatcher(FakeEngine(vocab=VOCAB), 4, 16)
+    with pytest.raises(ValueError):
+        cb.submit([1], 4, **kw)
+    assert cb.idle()
+    top = float(np.finfo(np.float32).max)
+    cb.submit([1], 4, presence=top, frequency=-top, logit_bias={3: top, 4: -top, 5: 1e-300})

@@ -228,8 +228,10 @@ class ContinuousBatcher:
         if max_tokens > self._hist_cap:
             raise ValueError("max_tokens exceeds the sampler history capacity")
         bias = {int(t): float(v) for t, v in (logit_bias or {}).items()}
-        if any(not 0 <= t < self.vocab for t in bias) or not all(np.isfinite([presence, frequency, *bias.values()])):
-            raise ValueError("penalties and biases must be finite numbers, biases of tokens in the vocabulary")
+        with np.errstate(over="ignore"):  # (they act in float32)
+            values = np.array([presence, frequency, *bias.values()], np.float64).astype(np.float32)
+        if any(not 0 <= t < self.vocab for t in bias) or not np.isfinite(values).all():
+            raise ValueError("penalties and biases must be finite float32 numbers, biases of tokens in the vocabulary")
         if allowed is not None and not callable(allowed):
             allowed = self._allowed_ids(allowed)
             if not allowed.size:
