@@ -108,3 +108,31 @@ def test_numbers_that_float32_does_not_hold_are_refused(kw):
     assert cb.idle()
     top = float(np.finfo(np.float32).max)
     cb.submit([1], 4, presence=top, frequency=-top, logit_bias={3: top, 4: -top, 5: 1e-300})
+
+
+@pytest.mark.parametrize("ids", [np.arange(VOCAB) % 2 == 0, [True, False], [1.0, 2.0], np.array([3.5]), ["5"],
+                                 np.array([2 ** 63 + 4], np.uint64), [None]])
+def test_allowed_takes_token_ids_only(monkeypatch, ids):
+    """A mask of the vocabulary (or other things that are no ids) is refused, and
+    ends its request when a function gives it."""
+    cb = batcher(monkeypatch)
+    with pytest.raises(ValueError):
+        cb.submit([1], 4, allowed=ids)
+    assert cb.idle()
+    rid = cb.submit([1], 4, allowed=lambda out: ids)
+    assert cb._sample_rows(torch.zeros(1, VOCAB), [cb.waiting[0]], torch.zeros(1, dtype=torch.int32)).tolist() == [-1]
+    assert isinstance(cb.errors[rid], ValueError)
+
+
+def test_allowed_is_kept_as_it_was_given(monkeypatch):
+    cb = batcher(monkeypatch)
+    for ids in ({5, 7}, range(3), np.array([[9, 11]], np.uint8), [np.int32(4)], np.array([8], np.uint64)):
+        cb.submit([1], 4, allowed=ids)
+    mine = np.array([20, 30])
+    cb.submit([1], 4, allowed=mine)
+    mine[:] = VOCAB
+    got = [sorted(r.allowed.tolist()) for r in cb.waiting]
+    assert got == [[5, 7], [0, 1, 2], [9, 11], [4], [8], [20, 30]]
+    cb.submit([1], 4, allowed=lambda out: [])
+    assert cb._sample_rows(torch.zeros(1, VOCAB), [cb.waiting[-1]], torch.zeros(1, dtype=torch.int32)).tolist() == [-1]
+    assert not cb.errors

@@ -246,7 +246,10 @@ class ContinuousBatcher:
         return rid
 
     def _allowed_ids(self, ids) -> np.ndarray:
-        ids = np.asarray(list(ids) if not isinstance(ids, np.ndarray) else ids, dtype=np.int64).reshape(-1)
+        ids = np.asarray(list(ids) if not isinstance(ids, np.ndarray) else ids)
+        if ids.size and ids.dtype.kind not in "iu":  # (a mask of the vocabulary is not a list of ids)
+            raise ValueError("allowed tokens must be whole numbers: token ids")
+        ids = ids.astype(np.int64).reshape(-1)  # (a copy: the caller's array may change)
         if ids.size and (ids.min() < 0 or ids.max() >= self.vocab):
             raise ValueError("allowed token out of range")
         return ids
