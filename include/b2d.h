@@ -428,7 +428,8 @@ B2D_API b2d_status b2d_kv4_read(const b2d_kv4_cache* cache, const int32_t* pos_d
 /* Queries over the cache.  Strides in elements; a head's dims are contiguous. */
 typedef struct {
   const void* q; /* [n_rows][n_heads][d_head], B2D_BF16 or B2D_F16 */
-  void* out;     /* the same shape and type; rows of no sequence stay as they are */
+  void* out;     /* the same shape and type; rows of no sequence stay as they are.  q itself
+                    (with its strides), or apart from it */
   int64_t q_row, q_head, out_row, out_head;
   const int32_t* lens;    /* [n_seqs] positions in the cache (0: rows see nothing) */
   const int32_t* q_start; /* [n_seqs + 1] first row of each sequence; NULL: one row each */

@@ -156,3 +156,56 @@ def test_append_skips_a_row_past_the_table_with_its_query(cuda, n, dtype):
         kv4_append(pool, k, v, at, table, seq=rows, q=src, q_out=out, status=status, **kw)
         assert int(status.item()) == 0x203 and torch.equal(pool, want_pool) and torch.equal(out[good], want)
         assert torch.equal(out[~good], q[~good] if inplace else torch.full_like(q[~good], 9.0))
+
+
+@pytest.mark.parametrize("dtype,heads,n_kv,d,lens,rows", [
+    ("bf16", 16, 4, 64, [1, 17, 333, 0], None), ("f16", 10, 2, 128, [70, 5000], None),
+    ("f16", 8, 2, 128, [130, 77], [100, 77]), ("bf16", 8, 2, 64, [4097], [70])])
+def test_attention_onto_its_queries(cuda, dtype, heads, n_kv, d, lens, rows):
+    """out = q, contiguous and as a part of packed rows: what a separate out has."""
+    t, counts = TYPES[dtype], rows or [1] * len(lens)
+    n, bps = sum(counts), (max(lens) + 15) // 16
+    gen = torch.Generator().manual_seed(n + d)
+    pool, table = new_kv4_pool(len(lens) * bps, n_kv, d, cuda), i32(np.arange(len(lens) * bps).reshape(len(lens), bps), cuda)
+    for i, length in enumerate(lens):
+        k = torch.randn(length, n_kv, d, generator=gen).to(cuda)
+        kv4_append(pool, k, k, i32(np.arange(length), cuda), table, seq=i32(np.full(length, i), cuda))
+    packed = torch.randn(n, heads + 2 * n_kv, d, generator=gen).to(t).to(cuda)
+    q, rest = packed[:, :heads], packed[:, heads:].clone()
+    kw = dict(q_start=None if rows is None else i32(np.cumsum([0, *rows]), cuda))
+    want = kv4_attention(q, pool, i32(lens, cuda), table, **kw)
+    alone = q.contiguous()
+    for x in (alone, q):
+        assert kv4_attention(x, pool, i32(lens, cuda), table, out=x, **kw) is x and torch.equal(x, want)
+    assert torch.equal(packed[:, heads:], rest)
+
+
+def test_outputs_that_overlap_inputs_in_part_are_refused(cuda):
+    from transformer_b200.generate import adjust_logits
+    n, d = 4, 64
+    buf = torch.zeros(n + 1, 9, d, device=cuda)
+    q, k, v = buf[:n, :4], buf[:n, 4:6], buf[:n, 6:8]
+    pool, table, pos = new_kv4_pool(n, 2, d, cuda), i32(np.arange(n)[:, None], cuda), i32(np.zeros(n), cuda)
+    for out in (buf[1:, :4], buf[:n, 1:5], buf[:n, 4:8], buf.view(-1)[1:].as_strided((n, 4, d), q.stride()),
+                buf.view(-1).as_strided((n, 4, d), (5 * d, d, 1)), torch.zeros(n, 1, d, device=cuda).expand(n, 4, d),
+                buf.view(torch.bfloat16)[:n, :4, :d]):
+        with pytest.raises(ValueError):
+            kv4_append(pool, k, v, pos, table, q=q, q_out=out)
+    assert torch.count_nonzero(pool) == 0 and torch.count_nonzero(buf) == 0
+    for out in (q, torch.empty(n, 4, d, dtype=torch.float16, device=cuda)):
+        assert kv4_append(pool, k, v, pos, table, q=q, q_out=out) is out
+    h = torch.zeros(n + 1, 9, d, device=cuda, dtype=torch.bfloat16)
+    lens = i32(np.ones(n), cuda)
+    for out in (h[1:, :4], h[:n, 1:5], h.view(-1)[1:].as_strided((n, 4, d), h.stride()),
+                torch.zeros(1, 4, d, device=cuda, dtype=torch.bfloat16).expand(n, 4, d)):
+        with pytest.raises(ValueError):
+            kv4_attention(h[:n, :4], pool, lens, table, out=out)
+    kv4_attention(h[:n, :4], pool, lens, table, out=h[:n, 4:8])
+    flat = torch.zeros(300, device=cuda)
+    lg = flat.as_strided((3, 50), (100, 1))
+    for out in (flat[1:].as_strided((3, 50), (100, 1)), flat[100:].as_strided((2, 50), (100, 1)),
+                flat.as_strided((3, 50), (50, 1)), flat[49:].as_strided((3, 50), (100, 1))):
+        with pytest.raises(ValueError):
+            adjust_logits(lg[:out.shape[0]], out=out)
+    other = flat[50:].as_strided((3, 50), (100, 1))  # the other half of each row
+    assert adjust_logits(lg, out=other) is other and adjust_logits(lg, out=lg) is lg

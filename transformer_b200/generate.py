@@ -37,7 +37,7 @@ import torch
 
 from . import _lib
 from .config import ModelConfig
-from .kv4 import _empty_like, _stream_on
+from .kv4 import _empty_like, _overlap, _same_place, _stream_on
 from .multi_sm_decode import DecodeEngine, _ptr, _stream_ptr
 from .packing import prepare_decode_weights_nlayer
 
@@ -100,7 +100,8 @@ def adjust_logits(logits, *, out=None, history=None, hist_len=None, prompt_len=N
     if logits.dtype is not torch.float32 or logits.dim() != 2 or dev < 0:
         raise ValueError("logits must be float32 [batch, vocab] on a GPU")
     batch, vocab = shape = logits.shape
-    if out is None:
+    given = out is not None
+    if not given:
         out = _empty_like(logits, stream)
     ld, one = logits.stride()
     out_ld, out_one = out.stride() if out.dim() == 2 else (0, 0)
@@ -109,6 +110,8 @@ def adjust_logits(logits, *, out=None, history=None, hist_len=None, prompt_len=N
     if vocab < 1 or out.dtype is not torch.float32 or out.shape != shape or out.get_device() != dev or (
             vocab > 1 and (one != 1 or out_one != 1)) or ld < vocab or out_ld < vocab:
         raise ValueError("logits and out must be float32 [batch, vocab] on one GPU, their rows contiguous and apart")
+    if given and not _same_place(out, logits) and _overlap(out, logits):
+        raise ValueError("out must be the logits or apart from them")
     if (history is None) != (hist_len is None):
         raise ValueError("history and hist_len go together")
     if history is None and not (prompt_len is None and rep_penalty is None and presence is None and frequency is None):

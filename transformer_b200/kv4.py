@@ -19,6 +19,7 @@ from __future__ import annotations
 import ctypes
 import functools
 
+import numpy as np
 import torch
 
 from . import _lib
@@ -99,6 +100,53 @@ def _strides(t, name, index, shape, types):
     return t.data_ptr(), row, head
 
 
+def _starts(x) -> np.ndarray:
+    """Sorted addresses of the contiguous pieces (last dim) of x."""
+    at = np.zeros(1, np.int64)
+    for size, stride in zip(x.shape[:-1], x.stride()[:-1]):
+        at = (at[:, None] + np.arange(size) * stride).reshape(-1)
+    return np.sort(x.data_ptr() + at * x.element_size())
+
+
+def _overlap(x, y) -> bool:
+    """Whether tensors of any outer strides (contiguous in their last dim) share a byte."""
+    if not x.numel() or not y.numel():
+        return False
+    xs, ys = x.element_size(), y.element_size()
+    xp, yp, x_shape, y_shape, x_str, y_str = x.data_ptr(), y.data_ptr(), x.shape, y.shape, x.stride(), y.stride()
+    if (yp >= xp + xs * sum([(n - 1) * s for n, s in zip(x_shape, x_str)], 1)
+            or xp >= yp + ys * sum([(n - 1) * s for n, s in zip(y_shape, y_str)], 1)):
+        return False
+    # views of one buffer's rows, side by side
+    row = xs * x_str[0]
+    x_row, y_row = (e * sum([(n - 1) * s for n, s in zip(shape[1:], st[1:])], 1)
+                    for e, shape, st in ((xs, x_shape, x_str), (ys, y_shape, y_str)))
+    if row == ys * y_str[0] and row > 0:
+        off = (yp - xp) % row
+        if off >= x_row and off + y_row <= row:
+            return False
+    a, b = _starts(x), _starts(y)
+    x_len, y_len = xs * x_shape[-1], ys * y_shape[-1]
+    return bool((np.searchsorted(b, a + x_len, "left") > np.searchsorted(b, a - y_len, "right")).any())
+
+
+def _same_place(x, y) -> bool:
+    """Whether tensors of one shape and type have the same elements."""
+    return x.data_ptr() == y.data_ptr() and all(n < 2 or s == t for n, s, t in zip(x.shape, x.stride(), y.stride()))
+
+
+def _folded(x) -> bool:
+    """Whether two elements of x share their place."""
+    need = 1
+    for stride, size in sorted((s, n) for s, n in zip(x.stride(), x.shape) if n > 1):
+        if stride < need:
+            break
+        need = stride * size
+    else:
+        return False
+    return bool(x.numel()) and bool((np.diff(_starts(x)) < x.shape[-1] * x.element_size()).any())
+
+
 @functools.lru_cache(maxsize=4096)
 def _scratch_bytes(index, n_kv, d, heads, n_seqs, max_rows, max_len) -> int:
     """Bytes of scratch that a call of these sizes needs (a function of them alone)."""
@@ -139,13 +187,15 @@ def kv4_append(pool, k, v, pos, table, *, seq=None, q=None, q_out=None, cos=None
         q_ptr, q_row, q_head = _strides(q, "q", dev, (n, heads, d), (k.dtype,))
         if heads < 1:
             raise ValueError("q needs a head")
-        if q_out is None:
+        given = q_out is not None
+        if not given:
             q_out = _empty_like(q, stream)
         o_ptr, o_row, o_head = _strides(q_out, "q_out", dev, (n, heads, d),
                                         _TYPES if q.dtype is torch.float32 else (q.dtype,))
         o_type = _TYPES[q_out.dtype]
-        if o_ptr == q_ptr and n and (o_row != q_row or o_head != q_head or o_type != dtype):
-            raise ValueError("q_out must be q or apart from it")
+        if given and (_folded(q_out) or _overlap(q_out, k) or _overlap(q_out, v) or (
+                not (o_type == dtype and _same_place(q_out, q)) and _overlap(q_out, q))):
+            raise ValueError("q_out must be q or apart from it, and apart from k and v")
     elif q_out is not None:
         raise ValueError("q_out without q")
     if (cos is None) != (sin is None):
@@ -197,7 +247,8 @@ _QUERY_TYPES = (torch.bfloat16, torch.float16)
 def kv4_attention(q, pool, lens, table, *, q_start=None, max_rows=None, max_len=None, scale=None, out=None,
                   status=None, stream=None):
     """Causal attention of the rows ``q`` [n, heads, d] (bf16 or fp16) over the
-    4-bit cache; returns ``out`` (default: a new tensor of q's shape and type).
+    4-bit cache; returns ``out`` (default: a new tensor of q's shape and type;
+    may be ``q``).
 
     Sequence i (row i of ``table``) has ``lens[i]`` positions in the cache
     (int32; 0: its rows see nothing and become 0).  Decode: one row a
@@ -215,9 +266,12 @@ def kv4_attention(q, pool, lens, table, *, q_start=None, max_rows=None, max_len=
     n_seqs = lens.numel()
     if n_seqs > table_rows:
         raise ValueError("more lengths than table rows")
-    if out is None:
+    given = out is not None
+    if not given:
         out = _empty_like(q, stream)
     o_ptr, o_row, o_head = _strides(out, "out", dev, shape, (q.dtype,))
+    if given and (_folded(out) or (not _same_place(out, q) and _overlap(out, q))):
+        raise ValueError("out must be q or apart from it")
     room = min(bps * PAGE_TOKENS, 2 ** 31 - 1)
     max_len = room if max_len is None else int(max_len)
     if not 0 <= max_len <= room:
