@@ -62,3 +62,27 @@ def test_rules_and_repetition_together(engine_tiny_batched, pipeline):
     engine_tiny_batched.check_device()
     assert not wrong, wrong[:5]
     assert seen == sum(map(len, got.values())) == 8 * 30
+
+
+def test_lists_without_room(cuda):
+    """A history and biases of no entries (the first step of a batch) change
+    nothing; lists that are no matrices are refused."""
+    import torch
+    from transformer_b200.generate import adjust_logits
+    lg = torch.randn(3, 70, device=cuda)
+    zero, one = torch.zeros(3, dtype=torch.int32, device=cuda), torch.ones(3, device=cuda)
+    none = torch.zeros(3, 0, dtype=torch.int32, device=cuda)
+    kw = dict(history=none, hist_len=zero, prompt_len=zero, rep_penalty=2 * one, presence=one, frequency=one)
+    assert torch.equal(adjust_logits(lg, **kw), lg)
+    bias = dict(bias_ids=none, bias_values=none.float(), bias_len=zero)
+    assert torch.equal(adjust_logits(lg, **bias, **kw), lg)
+    allowed = torch.full((3, 3), 6, dtype=torch.int32, device=cuda)
+    got = adjust_logits(lg, **bias, **kw, allowed=allowed)
+    keep = torch.arange(70, device=cuda) % 32
+    keep = (keep == 1) | (keep == 2)
+    assert torch.equal(got[:, keep], lg[:, keep]) and torch.isneginf(got[:, ~keep]).all()
+    for bad in (dict(history=zero[0], hist_len=zero), dict(allowed=zero[0]), dict(history=none, hist_len=zero[:2]),
+                dict(bias_ids=none, bias_values=none, bias_len=zero),
+                dict(bias_ids=zero, bias_values=one, bias_len=zero)):
+        with pytest.raises(ValueError):
+            adjust_logits(lg, **bad)

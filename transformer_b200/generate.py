@@ -119,9 +119,7 @@ def adjust_logits(logits, *, out=None, history=None, hist_len=None, prompt_len=N
     if (bias_ids is None) != (bias_values is None) or (bias_ids is None) != (bias_len is None):
         raise ValueError("bias_ids, bias_values and bias_len go together")
     row = (batch,)
-    cap = history.shape[-1] if history is not None else 0
-    n_bias = bias_ids.shape[-1] if bias_ids is not None else 0
-    words = allowed.shape[-1] if allowed is not None else 0
+    cap, n_bias, words = (t.shape[1] if t is not None and t.dim() == 2 else 0 for t in (history, bias_ids, allowed))
     if allowed is not None and 32 * words < vocab:
         raise ValueError(f"allowed must have {(vocab + 31) // 32} words a row")
 
@@ -133,13 +131,17 @@ def adjust_logits(logits, *, out=None, history=None, hist_len=None, prompt_len=N
         return t.data_ptr()
 
     i32, f32 = torch.int32, torch.float32
-    r = _lib.LogitsRules(
-        logits.data_ptr(), out.data_ptr(), ld, out_ld, take(history, "history", i32, (batch, cap)),
-        take(hist_len, "hist_len", i32, row), take(prompt_len, "prompt_len", i32, row),
-        take(rep_penalty, "rep_penalty", f32, row), take(presence, "presence", f32, row),
-        take(frequency, "frequency", f32, row), take(bias_ids, "bias_ids", i32, (batch, n_bias)),
-        take(bias_values, "bias_values", f32, (batch, n_bias)), take(bias_len, "bias_len", i32, row),
-        take(allowed, "allowed", i32, (batch, words)), words, batch, vocab, cap, n_bias, dev)
+    seen = [take(history, "history", i32, (batch, cap)), take(hist_len, "hist_len", i32, row),
+            take(prompt_len, "prompt_len", i32, row), take(rep_penalty, "rep_penalty", f32, row),
+            take(presence, "presence", f32, row), take(frequency, "frequency", f32, row)]
+    bias = [take(bias_ids, "bias_ids", i32, (batch, n_bias)), take(bias_values, "bias_values", f32, (batch, n_bias)),
+            take(bias_len, "bias_len", i32, row)]
+    if not cap:  # (lists without room have no address: as none)
+        seen = [None] * 6
+    if not n_bias:
+        bias = [None] * 3
+    r = _lib.LogitsRules(logits.data_ptr(), out.data_ptr(), ld, out_ld, *seen, *bias,
+                         take(allowed, "allowed", i32, (batch, words)), words, batch, vocab, cap, n_bias, dev)
     if batch:
         _lib.check(_lib.load().b2d_adjust_logits(ctypes.byref(r), _stream_on(stream, dev)), "b2d_adjust_logits")
     return out
