@@ -209,3 +209,32 @@ def test_outputs_that_overlap_inputs_in_part_are_refused(cuda):
             adjust_logits(lg[:out.shape[0]], out=out)
     other = flat[50:].as_strided((3, 50), (100, 1))  # the other half of each row
     assert adjust_logits(lg, out=other) is other and adjust_logits(lg, out=lg) is lg
+
+
+@pytest.mark.parametrize("dtype,heads,n_kv,d", [("bf16", 16, 4, 64), ("f16", 12, 6, 128)])
+def test_attention_of_many_short_chunks(cuda, dtype, heads, n_kv, d):
+    """More sequences and kv heads than SMs, each with one tile of 128 columns,
+    some with few rows, none, or more than positions."""
+    rng = np.random.default_rng(d)
+    n_seqs, bps, top = 45, 9, 128 // (heads // n_kv)
+    rows = rng.integers(0, top + 1, n_seqs)
+    lens = np.minimum(rows + rng.integers(-3, 90, n_seqs).clip(-3), 16 * bps).clip(0)
+    rows[:3], lens[:3] = (top, 0, top), (16 * bps, 20, 0)
+    pool, table = new_kv4_pool(n_seqs * bps, n_kv, d, cuda), i32(rng.permutation(n_seqs * bps).reshape(n_seqs, bps), cuda)
+    at, seq = i32(np.concatenate([np.arange(x) for x in lens]), cuda), i32(np.repeat(np.arange(n_seqs), lens), cuda)
+    k, v = (torch.from_numpy(rng.normal(size=(int(lens.sum()), n_kv, d)).astype(np.float32)).to(cuda) for _ in range(2))
+    kv4_append(pool, k, v, at, table, seq=seq)
+    held = [f64(x) for x in kv4_read(pool, at, table, seq=seq, dtype=torch.float32)]
+    q = torch.from_numpy(rng.normal(size=(int(rows.sum()), heads, d))).to(TYPES[dtype]).to(cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = kv4_attention(q, pool, i32(lens, cuda), table, q_start=i32(np.cumsum([0, *rows]), cuda), max_rows=top,
+                        status=status)
+    check_status(status)
+    a = b = 0
+    for n, c in zip(lens, rows):
+        hk, hv = (x[b:b + n] for x in held)
+        want, mass, size = R.attention(f64(q)[a:a + c], hk, hv, d ** -0.5)
+        bound = R.attention_bound(want, mass, size, max(n, 1), d, torch.finfo(TYPES[dtype]).eps / 2,
+                                  np.abs(hv).max(initial=0))
+        assert (np.abs(f64(out)[a:a + c] - want) <= bound).all()
+        a, b = a + c, b + n

@@ -145,8 +145,10 @@ bool kv4_attn_plan(Kv4AttnArgs& a, int sms) {
   a.tiles = static_cast<int>((cols + a.tile_cols - 1) / a.tile_cols);
   // Two groups of columns a CTA share the halves of K and V: where one each would
   // leave no SM without a CTA (288 tiles of 128 columns on 8192 positions: 147 us,
-  // and 212 with a group a CTA; 144 tiles: 126 and 111).
-  if (prompt && plan_units(a) > sms) {
+  // and 212 with a group a CTA; 144 tiles: 126 and 111).  One tile of a sequence and
+  // kv head has nobody to share with (256 of them on 4096 positions: 130 us a group a
+  // CTA, 154 in pairs of which one is empty; on 512, 33 and 34).
+  if (prompt && a.tiles > 1 && plan_units(a) > sms) {
     a.tile_cols *= 2;
     a.tiles = (a.tiles + 1) / 2;
   }
