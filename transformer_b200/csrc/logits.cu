@@ -131,9 +131,12 @@ extern "C" b2d_status b2d_adjust_logits(const b2d_logits_rules* r, void* stream)
     return B2D_ERR_INVALID_ARG;
   if (r->batch > 65535) return B2D_ERR_UNSUPPORTED;
   if (r->batch == 0) return B2D_OK;
-  // whole slices where the rows fill the GPU (two CTAs to each of 148 SMs); a few rows are cut finer
+  int sms = 0;
+  const cudaError_t got = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, r->device);
+  if (got != cudaSuccess) return b2d::cuda_failed(got, "SM count");
+  // whole slices where the rows fill the GPU (two CTAs to each SM); a few rows are cut finer
   int slice = b2d::kLogitsSlice;
-  while (slice > b2d::kLogitsThreads * 4 && int64_t(r->batch) * ((int64_t(r->vocab) + slice - 1) / slice) < 2 * 148) slice /= 2;
+  while (slice > b2d::kLogitsThreads * 4 && int64_t(r->batch) * ((int64_t(r->vocab) + slice - 1) / slice) < 2 * sms) slice /= 2;
   b2d::DeviceScope dev(r->device);
   if (dev.error() != cudaSuccess) return b2d::cuda_failed(dev.error(), "device");
   const dim3 grid(static_cast<unsigned>((int64_t(r->vocab) + slice - 1) / slice), static_cast<unsigned>(r->batch));
