@@ -55,3 +55,25 @@ def test_empty_and_equal_views():
     assert not _folded(buf[:, 1:, :2]) and _folded(buf[:1].expand(3, 6, 4))
     assert _same_place(buf, buf.view(8, 6, 4)) and _same_place(buf[:1], buf[0].as_strided((1, 6, 4), (99, 4, 1)))
     assert not _same_place(buf[:, :2], buf.view(16, 3, 4)[:8, :2])
+
+
+def test_a_pool_off_16_bytes_is_refused():
+    """Its pages are copied 16 bytes at a time; a view that starts between is
+    refused on the host."""
+    import types
+
+    from transformer_b200.config import CONFIG_TINY as cfg
+    from transformer_b200.kv4 import page_bytes
+    from transformer_b200.multi_sm_decode import DecodeEngine
+    eng = types.SimpleNamespace(cfg=cfg, kv_bits=4, device=torch.device("cpu"))
+    shape = (cfg.n_layers, 3, cfg.n_kv_heads, page_bytes(cfg.d_head))
+    size = 3 * cfg.n_layers * cfg.n_kv_heads * page_bytes(cfg.d_head)
+    buf = torch.zeros(size + 64, dtype=torch.uint8)
+    base = -buf.data_ptr() % 16
+    for off in range(17):
+        pool = buf[base + off:base + off + size].view(shape)
+        if off % 16:
+            with pytest.raises(ValueError):
+                DecodeEngine._check_pool(eng, pool)
+        else:
+            DecodeEngine._check_pool(eng, pool)

@@ -916,6 +916,8 @@ namespace {
 b2d_status run_rows(b2d_model* m, b2d_ws* ws, const int32_t* tok, const int32_t* pos, int batch, void* cache,
                     const int32_t* table, int bps, int num_blocks, bool prefill, float* logits, int32_t* next_tok,
                     cudaStream_t st, int out_tail = 0, int table_ld = -1) {
+  // (pages of a 4-bit pool come by copies of 16 bytes)
+  if (ws->kv4 && table && (reinterpret_cast<uintptr_t>(cache) & 15u)) return B2D_ERR_INVALID_ARG;
   b2d_status s = ensure_weight_maps(m);
   if (s != B2D_OK) return s;
   const b2d_config& c = m->cfg;

@@ -177,8 +177,9 @@ class DecodeEngine:
         c = self.cfg
         if self.kv_bits == 4:
             if (pool.dtype != torch.uint8 or pool.device != self.device or not pool.is_contiguous() or pool.dim() != 4
-                    or tuple(pool.shape[i] for i in (0, 2, 3)) != (c.n_layers, c.n_kv_heads, page_bytes(c.d_head))):
-                raise ValueError("pool must be a 4-bit paged KV pool of this model (see new_kv_pool)")
+                    or tuple(pool.shape[i] for i in (0, 2, 3)) != (c.n_layers, c.n_kv_heads, page_bytes(c.d_head))
+                    or pool.data_ptr() % 16):
+                raise ValueError("pool must be a 4-bit paged KV pool of this model (see new_kv_pool), 16-byte aligned")
             return
         if (pool.dtype != torch.bfloat16 or pool.device != self.device or not pool.is_contiguous() or pool.dim() != 6
                 or tuple(pool.shape[i] for i in (0, 2, 3, 4, 5)) != (c.n_layers, 2, c.n_kv_heads, PAGE_TOKENS,
