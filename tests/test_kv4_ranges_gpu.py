@@ -238,3 +238,36 @@ def test_attention_of_many_short_chunks(cuda, dtype, heads, n_kv, d):
                                   np.abs(hv).max(initial=0))
         assert (np.abs(f64(out)[a:a + c] - want) <= bound).all()
         a, b = a + c, b + n
+
+
+@pytest.mark.parametrize("n", [300, 512, 1024])  # (few rows, and a warp a row from 8 d on)
+@pytest.mark.parametrize("q_type", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("d,rotary", [(64, 64), (64, 32), (128, 128)])
+def test_append_of_float32_rows(cuda, n, q_type, d, rotary):
+    """What a model's pass of prompts appends: float32 rows of a packed
+    projection, queries into another type, the halves of a head rotated."""
+    heads, n_kv, t = 5, 2, TYPES.get(q_type, torch.float32)
+    gen = torch.Generator().manual_seed(n + d + rotary)
+    x = torch.randn(n, heads + 2 * n_kv, d, generator=gen).to(cuda)
+    q, k, v = x[:, :heads], x[:, heads:heads + n_kv], x[:, heads + n_kv:]
+    ang = torch.randn(n, rotary // 2, generator=gen)
+    cos, sin = ang.cos().to(cuda), ang.sin().to(cuda)
+    pages = (n + 15) // 16
+    rng = np.random.default_rng(n)
+    pool, table = new_kv4_pool(pages, n_kv, d, cuda), i32(rng.permutation(pages)[None], cuda)
+    order = rng.permutation(n)
+    pos, seq = i32(order, cuda), i32(np.zeros(n), cuda)
+    status = torch.zeros(1, dtype=torch.int32, device=cuda)
+    out = torch.empty(n, heads, d, dtype=t, device=cuda)
+    kv4_append(pool, k, v, pos, table, seq=seq, q=q, q_out=out, cos=cos, sin=sin, status=status)
+    check_status(status)
+    c, s = f64(cos)[order], f64(sin)[order]
+    got_k, got_v = kv4_read(pool, pos, table, seq=seq, dtype=torch.float32)
+    assert np.array_equal(f64(got_k), R.held(R.turned(f64(k), c, s, False)))
+    assert np.array_equal(f64(got_v), R.held(f64(v)))
+    # two products and a sum in float32 (3 2^-24 of |x| + |partner|), then one rounding
+    # (an fp16 one is off by up to 2^-25 however small the number)
+    want, pair = R.turned(f64(q), c, s, False), 2 * np.abs(f64(q)).max(-1, keepdims=True)
+    work = 3 * 2.0 ** -24 * pair
+    bound = torch.finfo(t).eps / 2 * (np.abs(want) + work) + work + (2.0 ** -25 if q_type == "f16" else 0.0)
+    assert (np.abs(f64(out) - want) <= bound).all()
