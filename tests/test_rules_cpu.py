@@ -136,3 +136,12 @@ def test_allowed_is_kept_as_it_was_given(monkeypatch):
     cb.submit([1], 4, allowed=lambda out: [])
     assert cb._sample_rows(torch.zeros(1, VOCAB), [cb.waiting[-1]], torch.zeros(1, dtype=torch.int32)).tolist() == [-1]
     assert not cb.errors
+
+
+@pytest.mark.parametrize("bias", [{3.7: 1.0}, {"5": 1.0}, {True: 1.0}, {np.float32(2): 1.0}, {None: 0.0}])
+def test_biases_take_token_ids_only(bias):
+    cb = ContinuousBatcher(FakeEngine(vocab=VOCAB), 4, 16)
+    with pytest.raises(ValueError):
+        cb.submit([1], 4, logit_bias=bias)
+    cb.submit([1], 4, logit_bias={np.int32(3): 1, 4: np.float32(0.5)})
+    assert cb.waiting[0].logit_bias == {3: 1.0, 4: 0.5} and len(cb.waiting) == 1

@@ -227,6 +227,8 @@ class ContinuousBatcher:
             raise ValueError("bad sampling parameters")
         if max_tokens > self._hist_cap:
             raise ValueError("max_tokens exceeds the sampler history capacity")
+        if any(isinstance(t, (bool, np.bool_)) or not isinstance(t, (int, np.integer)) for t in logit_bias or {}):
+            raise ValueError("logit_bias must name tokens by their ids")
         bias = {int(t): float(v) for t, v in (logit_bias or {}).items()}
         with np.errstate(over="ignore"):  # (they act in float32)
             values = np.array([presence, frequency, *bias.values()], np.float64).astype(np.float32)
