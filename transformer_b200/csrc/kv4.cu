@@ -200,13 +200,14 @@ b2d_status check_cache(const b2d_kv4_cache* c, b2d::Kv4Cache& k) {
   return B2D_OK;
 }
 
+constexpr float kLog2e = 1.4426950408889634f;  // (exponents are of 2)
 b2d_status check_query(const b2d_kv4_cache* c, const b2d_kv4_query* q, b2d::Kv4AttnArgs& a) {
   std::memset(&a, 0, sizeof(a));
   const b2d_status s = check_cache(c, a.c);
   if (s != B2D_OK) return s;
   if (!q || !q->q || !q->out || !q->lens || q->n_rows < 0 || q->n_seqs < 0 || q->n_heads < 1 ||
       q->n_heads % c->n_kv_heads || q->max_rows < 1 || q->n_seqs > c->table_rows || q->max_len < 0 ||
-      int64_t(q->max_len) > int64_t(c->blocks_per_seq) * b2d::kKv4Page || !(q->scale > 0.f) || std::isinf(q->scale) ||
+      int64_t(q->max_len) > int64_t(c->blocks_per_seq) * b2d::kKv4Page || !(q->scale > 0.f) || std::isinf(q->scale * kLog2e) ||
       (!q->q_start && (q->n_rows != q->n_seqs || q->max_rows != 1)))
     return B2D_ERR_INVALID_ARG;
   if (q->dtype != B2D_BF16 && q->dtype != B2D_F16) return B2D_ERR_UNSUPPORTED;
@@ -216,7 +217,7 @@ b2d_status check_query(const b2d_kv4_cache* c, const b2d_kv4_query* q, b2d::Kv4A
   a.o_row = q->out_row; a.o_head = q->out_head;
   a.lens = q->lens;
   a.q_start = q->q_start;
-  a.scale_log2 = q->scale * 1.4426950408889634f;
+  a.scale_log2 = q->scale * kLog2e;
   a.n_rows = q->n_rows;
   a.n_heads = q->n_heads;
   a.n_seqs = q->n_seqs;
