@@ -132,7 +132,8 @@ B2D_API b2d_status b2d_workspace_create(b2d_model* m, int max_batch, b2d_ws** ou
 B2D_API b2d_status b2d_workspace_destroy(b2d_ws* ws);
 /* What the paged pools given with this workspace hold: bits 16 (default), bf16
  * values as b2d_decode_step_paged describes; bits 4, the 4-bit format below,
- * uint8 [n_layers][num_blocks][n_kv_heads][18 * d_head], 16-byte aligned.
+ * uint8 [n_layers][num_blocks][n_kv_heads][18 * d_head], 16-byte aligned (and the
+ * turned queries are rounded to bf16).
  * b2d_decode_step_paged, b2d_prefill_paged and b2d_prefill_rows follow it.
  * The first switch to 4 allocates, so it comes before any capture. */
 B2D_API b2d_status b2d_workspace_kv_bits(b2d_ws* ws, int bits);

@@ -1021,7 +1021,10 @@ b2d_status run_rows(b2d_model* m, b2d_ws* ws, const int32_t* tok, const int32_t*
   auto* att_k4 = att_tma ? b2d::paged_attn_mma_kernel<4, true> : b2d::paged_attn_mma_kernel<4, false>;
   const int att_smem2 = b2d::pa_smem_bytes(2, att_tma, att_stages);
   // 4-bit pool: the rows are turned, quantised and appended, then attend; a
-  // prompt's rows (one table row for all) as the chunk of one sequence.
+  // prompt's rows (one table row for all) as the chunk of one sequence, rows with a
+  // table row each as sequences of one row.  The turned queries go out in bf16, the
+  // type of the step's other activations (the 16-bit path holds them to 2^-17, next
+  // to keys of 8 bits; halves would have 3 bits more here and end at 65504).
   b2d::Kv4AppendArgs ka{};
   b2d::Kv4AttnArgs kt{};
   if (kv4) {

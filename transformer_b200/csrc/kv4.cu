@@ -17,7 +17,7 @@ namespace {
 template <class T, class TQ>
 cudaError_t append_typed(const Kv4AppendArgs& a, cudaStream_t st, bool pdl) {
   // Many rows: a warp takes a whole row, so its addresses and angles are worked
-  // out once (10242 rows of 48 heads of 128: 98 us with the read-back, 108 with
+  // out once (10239 rows of 48 heads of 128: 98 us with the read-back, 108 with
   // four warps a row); few: a block per batch of heads, one head a thread.  Rows
   // of 48 heads of 128, of 24 of 64 (us, few and many): 512 10.2 and 15.6, 5.7 and
   // 5.7; 1024 16.8 and 17.0, 9.3 and 7.4; 2000 30.3 and 20.8, 15.8 and 8.4.
@@ -116,7 +116,7 @@ int64_t plan_units(const Kv4AttnArgs& a) { return static_cast<int64_t>(a.n_seqs)
 // Splits: at least 32 pages each (8 a warp).  One sequence's splits are alike:
 // one wave of CTAs, four to an SM (131071 positions, 8 kv heads of 128: 46 us,
 // and 55 us with splits for four waves).  Several sequences differ in length:
-// four waves even that out (32 of 1001 to 16384: 91 us, and 110 us with one).
+// four waves even that out (32 of 1001 to 16384: 93 us, and 110 us with one).
 // Prompts: one CTA to an SM, 64 pages each at least (256 rows of 4 heads on 8192
 // positions, 64 tiles: 69 us, and 109 without splits).
 int64_t plan_splits(const Kv4AttnArgs& a, int sms) {

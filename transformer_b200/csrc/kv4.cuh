@@ -226,7 +226,7 @@ __device__ __forceinline__ uint32_t kv4_quantise(const float (&hi)[8], const flo
     codes = codes * 16u + ((t & 1u) ? u : t);
   }
   codes -= 0x4B400000u * 0x11111111u;  // each number's bits are 0x4B400000 + 8 + n
-  // zero and capped scales (a NaN has the capped byte), and what the low parts decide, are for below
+  // zero scales (a NaN's byte is 0) and capped ones, and what the low parts decide, are for below
   const bool sure = b - 1u < kKv4MaxByte - 1u && (few || (differ == 0u && 7.f * s != m));
   if (__all_sync(0xffffffffu, sure)) return b;
   m = 0.f;
@@ -304,9 +304,11 @@ __device__ __forceinline__ void kv4_values(uint32_t w, const Kv4ScaleBf& k, uint
 // the heads it walks.  Reads and writes of rows are 16 bytes a lane, contiguous
 // over a head.  blockIdx.x = row; gridDim.y = 1: a block takes the whole row;
 // else blockIdx.y = a batch of query heads, one a thread, then K, then V.
-// 10242 rows of 32 + 8 + 8 heads of 128 (252 MB with the read-back): 80 us, and
-// 18 us to read the rows back; the instructions of the rotation and of deciding
-// codes bound it (2 a cycle and SM), not memory, whose share is 36 us.
+// 10239 rows of 32 + 8 + 8 heads of 128 (224 MB): 80 us, 34 at the copy rate.
+// No unit is full (47% of the issue slots, 29% of DRAM): a warp's chain of loads,
+// rotation, codes and stores bounds it, and registers how many of them it has in
+// flight (two query heads; rows of float32, as the engine's, already spill some
+// 60 bytes a thread: 512 of 16 + 4 + 4 heads of 64 5.1 us, 0.7 at the copy rate).
 constexpr int kKv4AppendThreads = 128;  // at most; one warp a row where there are many rows (see kv4.cu)
 
 // How the first `rotary` dims of a head pair up.
@@ -500,7 +502,9 @@ __global__ void __launch_bounds__(kKv4AppendThreads, 6) kv4_append_kernel(
 // ---- read --------------------------------------------------------------------------
 // Rows out of the cache as values (zeros where the position is negative or the
 // table names no page).  Block: 128 threads on one row; thread = 8 dims of a
-// kv head's K or V.
+// kv head's K or V.  10239 rows of 8 heads of 128 (54 MB): 14.8 us, 3.6 TB/s, of
+// the 8.2 that the copy rate gives: position, table and page are loads that wait
+// for one another, and a block has one row's.
 template <class T>
 __global__ void __launch_bounds__(128) kv4_read_kernel(const __grid_constant__ Kv4ReadArgs a) {
   pdl_wait();
@@ -548,9 +552,11 @@ __global__ void __launch_bounds__(128) kv4_read_kernel(const __grid_constant__ K
 // Both operands of both products are exact but for the probabilities: held
 // values are exact in bf16 and in half, so S is formed in the queries' own type
 // (as halves under a power of two per column, bf16 queries lost what lies 2^17
-// below their row's largest, and a wave of 256 took 14.5 us, not 13.9) and O in half.  Probabilities keep 11 bits: they
-// carry a factor 2^15, so those down to 2^-29 of the row's largest are normal
-// halves, and the sum they are divided by carries it too.
+// below their row's largest, and a wave of 256 took 14.5 us, not 13.9) and O in
+// half.  Probabilities keep 11 bits (as two halves they would double the second
+// product; a result of 8 bits hides it, one of 11 is off by up to a third more):
+// they carry a factor 2^15, so those down to 2^-29 of the row's largest are normal
+// halves, and the sum they are divided by, of the unrounded ones, carries it too.
 //
 // An exponent is the difference of two scores first, then scaled: scaled scores
 // apart, each rounded at its own size, would be off by more than the factor's room
@@ -758,8 +764,8 @@ constexpr __host__ __device__ int kv4_attn_smem() {
 // ring, kKv4Ahead steps ahead; a step takes P pages, so the running maximum
 // and the rescaling of o are paid once for 16 P positions.
 // One row of 32 heads over 8 of 128 dims on 131071 positions: 46 us with the join, 3.3
-// TB/s; 32 such rows on 1001 to 16384: 91 us, 3.5 TB/s.  Bound by instructions, 393 a
-// page of 2304 bytes, most of them turning codes to halves, at 64% of the issue slots.
+// TB/s; 32 such rows on 1001 to 16384: 93 us, 3.5 TB/s.  Bound by instructions, 386 a
+// page of 2304 bytes, most of them turning codes to values, at 62% of the issue slots.
 template <class T, int NH, int NB>
 __global__ void __launch_bounds__(32 * kKv4Warps) kv4_attn_kernel(const __grid_constant__ Kv4AttnArgs a) {
   constexpr int W = kKv4Warps, D = 64 * NH, COLS = 8 * NB, P = kv4_step_pages(NH), PB = kv4_page_bytes(D), SLOTS = kKv4Ahead + 1;

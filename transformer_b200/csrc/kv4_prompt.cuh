@@ -20,13 +20,14 @@
 // during the softmax of this one, O of the last one too.  One CTA to an SM.
 //
 // 4 chunks of 128 to 512 rows on 2049 to 8191 positions, 32 heads over 8 of 128
-// dims (125 GFLOP): 147 us, 845 TFLOP/s; 288 tiles of equal length 980.  What
-// bounds the latter: per tile and group the softmax has 512 cycles of exponentials
-// on a quarter SM, next to 250 of its other instructions and as many for the
-// codes; both products take 512 of the tensor cores (without the exponentials 130
-// instead of 147 us, without the codes 141, without most of the products 145).
-// The 4 chunks lose another 20% to the longest columns' end.  Measured on the
-// same case: two CTAs to an SM of one group, 205; four warps for K and V
+// dims (125 GFLOP): 153 us, 816 TFLOP/s; 288 tiles of equal length 151 us, 950.
+// What bounds the latter: per tile and group the softmax has 512 cycles of
+// exponentials on a quarter SM, next to 280 of its other instructions and as many
+// for the codes; both products take 512 of the tensor cores (before differences
+// and waits were made safe, 147 us: without the exponentials 130, without the codes
+// 141, without most of the products 145).  The 4 chunks lose another 20% to the
+// longest columns' end.  Measured on the same case when it took 147: two CTAs to
+// an SM of one group, 205; four warps for K and V
 // together, 166; all 64 scores held at once, 155; one pass with the last
 // maximum that is repeated when that was too small, 158; waits that poll, 147.
 // Before the longest came first, 274: tiles of 128 positions with one buffer 296
@@ -37,9 +38,10 @@
 // each 16, the positions of a page alike in S, P and V, and the dims of V, which
 // are O's columns, are put back on the way out.
 //
-// A column's running maximum is only moved, and O rescaled, when its scores
-// exceed it by 2^5 or more: P then stays below 2^15, and those down to 2^-24 of
-// the largest keep their 11 bits.
+// The softmax is the published online one (Milakov and Gimelshein, 2018) with a
+// maximum that may lag, as others have published since: it is only moved, and O
+// rescaled, when scores exceed it by 2^5 or more.  P then stays below 2^15, and
+// those down to 2^-24 of the largest keep their 11 bits.
 #pragma once
 
 #include <climits>

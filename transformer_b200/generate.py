@@ -80,7 +80,8 @@ def adjust_logits(logits, *, out=None, history=None, hist_len=None, prompt_len=N
     """Each row's own rules on a batch of logits (``b2d_adjust_logits``): what a
     request asks of its tokens before one is drawn.  ``logits``: float32
     [batch, vocab] on a GPU, rows contiguous; returns ``out`` (default: a new
-    tensor; ``logits`` itself adjusts in place).  Async, stream-ordered.
+    tensor; ``logits`` itself adjusts in place).  Async, stream-ordered
+    (``stream``: as in ``kv4``, the caller keeps the inputs until it is done).
 
     * ``history`` int32 [batch, cap] with ``hist_len`` int32 [batch]: the tokens
       of each row so far, of which the first ``prompt_len`` [batch] (default 0)

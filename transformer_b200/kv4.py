@@ -6,7 +6,10 @@ the functions here are its parts, for one layer's pool of any ``n_kv`` heads of
 of 16 dims with a scale of 8 bits, 4.5 bits a value, and held values exact in
 bf16 and fp16).  The reference has no cache below bf16.
 
-All calls are asynchronous and stream-ordered.  A pool is the uint8 tensor of
+All calls are asynchronous and stream-ordered.  ``stream``: a stream of the
+pool's device instead of the current one; the caller keeps the inputs (or
+records them on it) until it is done with them, and orders it behind what wrote
+them.  New outputs come from that stream's memory.  A pool is the uint8 tensor of
 ``new_kv4_pool``; a block of it holds 16 positions; ``table`` int32
 [n_seqs, blocks_per_seq] names the block of positions 16i.. of each sequence.
 Entries are read only where a position needs them.  Bad entries, positions and
