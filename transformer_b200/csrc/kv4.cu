@@ -143,7 +143,7 @@ bool kv4_attn_plan(Kv4AttnArgs& a, int sms) {
   const bool prompt = cols > 64 || (cols > 32 && work >= 1 << 16) || (cols > 16 && a.c.d == 128 && work >= 1 << 19);
   a.tile_cols = prompt ? kKv4PromptCols : cols <= 8 ? 8 : 16;
   a.tiles = static_cast<int>((cols + a.tile_cols - 1) / a.tile_cols);
-  // Two groups of columns a CTA share the halves of K and V: where one each would
+  // Two groups of columns a CTA share the values of K and V: where one each would
   // leave no SM without a CTA (288 tiles of 128 columns on 8192 positions: 147 us,
   // and 212 with a group a CTA; 144 tiles: 126 and 111).  One tile of a sequence and
   // kv head has nobody to share with (256 of them on 4096 positions: 130 us a group a

@@ -8,8 +8,8 @@
 //   O += P V    M = 128 columns, N = d, K = 64 positions; P in tensor memory, V in
 //               shared memory
 // with the operands of kv4.cuh (held values and queries exact, S in the queries'
-// type, P with 11 bits and a factor 2^10).  Its warps have parts, which meet only on mbarriers (for
-// two groups):
+// type, P with 11 bits and a factor 2^10).  Its warps have parts, which meet only
+// on mbarriers (for two groups):
 //   warps 0-7    softmax: thread r owns column r, lane r % 128 of its group's
 //                tensor memory
 //   warps 8-11   turn K's codes to values, a page of each tile, straight into the
